@@ -3,7 +3,8 @@
  *
  * The library behind this header (librecsdk_hip.so) implements, as hand-written HIP kernels, the
  * data-parallel path   key dedup -> admission -> key->slot hash table -> row gather / pooled lookup ->
- * gradient segment-reduce -> sparse optimizer update,   and nothing else.
+ * gradient segment-reduce -> sparse optimizer update,   and the training head over the looked-up rows
+ * (dropout, layer norm, softmax loss over an item table).
  *
  * Conventions
  *   - plain pointers and sizes only; `stream` is a hipStream_t passed as void* (NULL = default stream);
@@ -719,6 +720,67 @@ RECSDK_API int recsdk_tbe_backward_unique(recsdk_tbe_t* h, int32_t optim, const 
                                           const int64_t* d_unique_offsets, const int64_t* d_unique_inverse,
                                           int64_t num_unique, float* d_momentum1, float* d_momentum2, float lr,
                                           float eps, float beta1, float beta2, int64_t iter, void* stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * The training head over the looked-up rows: dropout, layer norm and the softmax loss over an item table, each with its
+ * backward pass.  No counterpart in the reference, whose models take these from their framework.  The calls hold no
+ * state: what a call needs beside its operands is a workspace of the caller's, whose contents nobody needs before or after
+ * (one workspace per call in flight).  No atomics on floating values: the same call gives the same bits.  Every call
+ * launches kernels only and may be recorded into a HIP graph. */
+
+/* Dropout with a mask that is a function of (seed, offset, element) and stored nowhere.  Element e of the n contiguous ones
+ * is kept where its 16 random bits are below B = round(65536 (1 - p)), and is then multiplied by 65536 / B (in fp32, rounded
+ * once); others become 0, whatever they held.  The bits: Philox-4x32-10 with key `seed` and counter (e / 8, offset), eight
+ * elements per block, the low half of each word first.  The backward pass is the same call on the gradient.
+ *   dtype    RECSDK_DT_F32, RECSDK_DT_F16 or RECSDK_DT_BF16
+ *   p        in [0, 1]; B = 0 drops everything
+ *   d_step   NULL, or a device word that is added to offset when the kernel runs: a replayed graph, whose scalar arguments
+ *            are fixed, draws a new mask where the caller advances the word
+ *   d_y      may be d_x */
+RECSDK_API int recsdk_dropout(const void* d_x, int64_t n, int32_t dtype, double p, uint64_t seed, uint64_t offset,
+                              const int64_t* d_step, void* d_y, void* stream);
+
+/* y = (x - mean) rstd weight + bias per row of dim columns, rstd = 1 / sqrt(var + eps), var the mean squared difference.
+ *   dtype      of x and y: RECSDK_DT_F32, RECSDK_DT_F16 or RECSDK_DT_BF16; w_dtype of weight and bias: dtype or RECSDK_DT_F32
+ *   x_stride   elements between rows of x (>= dim); y is contiguous and does not overlap x
+ *   d_weight, d_bias   [dim] or NULL (1 and 0);  d_mean, d_rstd  [rows] fp32 for the backward pass, or both NULL
+ * Statistics and sums are fp32.  Any dim; rows < 2^31. */
+RECSDK_API int recsdk_layer_norm_forward(const void* d_x, int64_t rows, int32_t dim, int64_t x_stride, int32_t dtype,
+                                         const void* d_weight, const void* d_bias, int32_t w_dtype, float eps, void* d_y,
+                                         float* d_mean, float* d_rstd, void* stream);
+/* Bytes of workspace that recsdk_layer_norm_backward takes for dweight / dbias (none for dx alone). */
+RECSDK_API int recsdk_layer_norm_workspace(int64_t rows, int32_t dim, int64_t* h_bytes);
+/* dx (contiguous, of dtype), dweight and dbias (of w_dtype, sums over the rows); each may be NULL.  d_grad is contiguous.
+ * rows = 0 leaves dweight and dbias zero.  d_workspace is 16-byte aligned. */
+RECSDK_API int recsdk_layer_norm_backward(const void* d_grad, const void* d_x, int64_t rows, int32_t dim, int64_t x_stride,
+                                          int32_t dtype, const void* d_weight, int32_t w_dtype, const float* d_mean,
+                                          const float* d_rstd, void* d_dx, void* d_dweight, void* d_dbias,
+                                          void* d_workspace, int64_t workspace_bytes, void* stream);
+
+/* Softmax cross entropy of `rows` rows x against every row of a table, the scores kept nowhere:
+ *   z[n][v] = scale x[n].table[v] + item_bias[v],  lse[n] = log sum_v exp z[n][v],  loss[n] = lse[n] - z[n][target[n]]
+ *   dtype          of x and table: RECSDK_DT_F32 or RECSDK_DT_BF16, as embedding tables are; dim in [1, 256]
+ *   x_stride, table_stride   elements between rows (>= dim): rows with optimizer state behind them are read in place
+ *   d_target       [rows]; a target outside [0, items) (a padding position, a key that was not admitted) makes a row of
+ *                  loss 0 that gives no gradient; its row of x may hold anything
+ *   d_item_bias    [items] fp32 or NULL; takes no gradient.  A value at or below -1e30 (-infinity among them) takes the
+ *                  item out: a free slot of the table, whose row may hold anything.  A row whose target is taken out
+ *                  (so also one that no item is left for) has loss +infinity and gives no gradient
+ *   d_loss, d_lse  [rows] fp32; d_lse is for the backward pass: log-sum-exp, or +infinity where a row gives no gradient
+ * d_x, d_table and d_workspace are 16-byte aligned.  Sums and statistics are fp32; bf16 probabilities are rounded to bf16
+ * where they enter the gradients' products.  rows and items < 2^30, items >= 1. */
+RECSDK_API int recsdk_softmax_loss_workspace(int64_t rows, int64_t items, int32_t dim, int32_t dtype, int64_t x_stride,
+                                             int64_t table_stride, int64_t* h_forward_bytes, int64_t* h_backward_bytes);
+RECSDK_API int recsdk_softmax_loss_forward(const void* d_x, int64_t rows, int64_t x_stride, const void* d_table, int64_t items,
+                                           int64_t table_stride, int32_t dim, int32_t dtype, const int64_t* d_target,
+                                           const float* d_item_bias, float scale, float* d_loss, float* d_lse, void* d_workspace,
+                                           int64_t workspace_bytes, void* stream);
+/* With G[n][v] = grad_loss[n] scale (exp(z[n][v] - lse[n]) - [v = target[n]]):  dx = G table [rows, dim],
+ * dtable = G' x [items, dim], contiguous, of dtype; either may be NULL.  Rows of items that are taken out get zeros. */
+RECSDK_API int recsdk_softmax_loss_backward(const float* d_grad_loss, const void* d_x, int64_t rows, int64_t x_stride,
+                                            const void* d_table, int64_t items, int64_t table_stride, int32_t dim, int32_t dtype,
+                                            const int64_t* d_target, const float* d_item_bias, float scale, const float* d_lse,
+                                            void* d_dx, void* d_dtable, void* d_workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

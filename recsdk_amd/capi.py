@@ -68,6 +68,22 @@ PROTOTYPES = {
     "recsdk_lazy_adam": (c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p, c_void_p, c_float,
                                    c_float, c_float, c_float, c_void_p]),
     "recsdk_sgd": (c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_float, c_float, c_void_p]),
+    "recsdk_dropout": (c_int32, [c_void_p, c_int64, c_int32, ctypes.c_double, ctypes.c_uint64, ctypes.c_uint64, c_void_p,
+                                 c_void_p, c_void_p]),
+    "recsdk_layer_norm_forward": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_void_p, c_int32,
+                                            c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "recsdk_layer_norm_workspace": (c_int32, [c_int64, c_int32, POINTER(c_int64)]),
+    "recsdk_layer_norm_backward": (c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_int64, c_int32, c_void_p, c_int32,
+                                             c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
+                                             c_void_p]),
+    "recsdk_softmax_loss_workspace": (c_int32, [c_int64, c_int64, c_int32, c_int32, c_int64, c_int64, POINTER(c_int64),
+                                                POINTER(c_int64)]),
+    "recsdk_softmax_loss_forward": (c_int32, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32, c_int32,
+                                              c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_int64,
+                                              c_void_p]),
+    "recsdk_softmax_loss_backward": (c_int32, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_int32,
+                                               c_int32, c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p,
+                                               c_int64, c_void_p]),
     "recsdk_unique_create": (c_int32, [c_int64, c_int32, POINTER(c_void_p)]),
     "recsdk_unique_destroy": (c_int32, [c_void_p]),
     "recsdk_unique_run": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int64,

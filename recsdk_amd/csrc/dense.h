@@ -1,0 +1,74 @@
+// Element types and small helpers shared by the dense kernels (dropout.hip, norm.hip, softmax_loss.hip).
+#ifndef RECSDK_CSRC_DENSE_H
+#define RECSDK_CSRC_DENSE_H
+
+#include "common.h"
+
+namespace recsdk {
+
+typedef uint32_t Word4 __attribute__((ext_vector_type(4)));   // 16 bytes as one lane moves them
+typedef float Float4 __attribute__((ext_vector_type(4)));
+
+// Bytes of a floating element type, 0 for anything else.
+inline int float_bytes(int32_t dtype)
+{
+    return dtype == RECSDK_DT_F32 ? 4 : (dtype == RECSDK_DT_F16 || dtype == RECSDK_DT_BF16) ? 2 : 0;
+}
+
+inline bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+#ifdef __HIPCC__
+
+using F16 = _Float16;
+using BF16 = __bf16;
+
+// Rounds to nearest even, as every store of a result does.
+template <typename T>
+__device__ __forceinline__ T from_float(float v)
+{
+    return (T)v;
+}
+
+// E elements of type T as they come from memory: one 16-byte access where E * sizeof(T) is 16, else element by element.
+template <typename T, int E>
+struct Pack {
+    T v[E];
+};
+
+template <typename T, int E>
+__device__ __forceinline__ Pack<T, E> load_pack(const T* p)
+{
+    Pack<T, E> r;
+    if constexpr (E * sizeof(T) == 16) {
+        const Word4 w = *reinterpret_cast<const Word4*>(p);
+        __builtin_memcpy(&r, &w, 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            r.v[e] = p[e];
+        }
+    }
+    return r;
+}
+
+// Streamed past the caches: results are written once and read by a later kernel.
+template <typename T, int E>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, E>& r)
+{
+    if constexpr (E * sizeof(T) == 16) {
+        Word4 w;
+        __builtin_memcpy(&w, &r, 16);
+        __builtin_nontemporal_store(w, reinterpret_cast<Word4*>(p));
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            p[e] = r.v[e];
+        }
+    }
+}
+
+#endif  // __HIPCC__
+
+}  // namespace recsdk
+
+#endif
