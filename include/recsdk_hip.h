@@ -767,7 +767,7 @@ RECSDK_API int recsdk_layer_norm_backward(const void* d_grad, const void* d_x, i
  *                  item out: a free slot of the table, whose row may hold anything.  A row whose target is taken out
  *                  (so also one that no item is left for) has loss +infinity and gives no gradient
  *   d_loss, d_lse  [rows] fp32; d_lse is for the backward pass: log-sum-exp, or +infinity where a row gives no gradient
- * d_x, d_table and d_workspace are 16-byte aligned.  Sums and statistics are fp32; bf16 probabilities are rounded to bf16
+ * d_x, d_table, d_workspace, and the gradients d_dx and d_dtable are 16-byte aligned.  Sums and statistics are fp32; bf16 probabilities are rounded to bf16
  * where they enter the gradients' products.  rows and items < 2^30, items >= 1. */
 RECSDK_API int recsdk_softmax_loss_workspace(int64_t rows, int64_t items, int32_t dim, int32_t dtype, int64_t x_stride,
                                              int64_t table_stride, int64_t* h_forward_bytes, int64_t* h_backward_bytes);

@@ -8,9 +8,9 @@
 // x goes by).  The three passes are one kernel: a wave OWNS 32 or 64 rows of one operand, held in registers as the
 // B operand of the matrix instruction, and the other operand STREAMS through LDS in tiles that the four waves of the
 // block share.  S = stream owner' has the owner's row in the lane and the stream's rows in the registers, so the
-// running sums need no exchange between lanes, and exp(S) is, as it lies, the A operand of the second product
-// (contracted over the stream's rows, 8 of 16 per half wave); the B operand of that product is the same LDS tile read
-// through the transposing LDS load.  A tile is laid out in 16-byte chunks whose place is exchanged by the row
+// running sums need no exchange between lanes, and exp(S) is, as it lies, the B operand of the second product
+// (contracted over the stream's rows, 8 of 16 per half wave); the A operand of that product is the same LDS tile read
+// through the transposing LDS load, so that a lane ends up with groups of four columns of its own row.  A tile is laid out in 16-byte chunks whose place is exchanged by the row
 // (`swizzle`), which keeps both kinds of read free of bank conflicts.
 //
 // float32 rows are split into three bfloat16 planes (8 + 8 + 8 bits of the mantissa) and a product of them is the six
@@ -23,6 +23,8 @@
 // leave partial sums in the workspace, which a second kernel joins in a fixed order: no atomics, a call gives the same
 // bits every time.
 #include <math.h>
+
+#include <type_traits>
 
 #include "dense.h"
 
@@ -39,13 +41,7 @@ constexpr float kFloor = -3e38f;         // running maximum before the first ite
 constexpr float kSlack = 10.0f;          // the running maximum may lag by a factor of 2^10
 constexpr int kLossThreads = 256;
 constexpr int kLossMaxDim = 256;
-
-struct Yes {
-    static constexpr bool value = true;
-};
-struct No {
-    static constexpr bool value = false;
-};
+constexpr int kLossMaxStride = 1 << 22;   // elements; 128 rows of a tile stay within 32-bit offsets
 
 enum LossPass { kLossForward = 0, kLossDx = 1, kLossDt = 2 };
 
@@ -71,19 +67,12 @@ struct LossArgs {
 
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 
-// Where chunk c (16 bytes) of tile row r lies within the row: the 16 rows that one access of the first product
-// touches, and the 4 rows by 4 chunks that one of the transposing loads touches, then fall on different banks.
-template <int CHUNKS>
-__device__ __forceinline__ int swizzle(int r, int c)
-{
-    if constexpr (CHUNKS >= 16) {
-        return c ^ (((r & 3) << 2) | ((r >> 2) & 3));
-    } else if constexpr (CHUNKS == 8) {
-        return c ^ ((((r >> 1) & 1) << 2) | ((r >> 2) & 3));
-    } else {
-        return c ^ ((r >> 2) & 3);
-    }
-}
+// Keeps what is derived from v next to its use: the compiler would move the comparisons' operands out of the loop and
+// hold them in registers for a branch that is hardly ever taken.
+__device__ __forceinline__ void pin(int& v) { asm volatile("" : "+v"(v)); }
+
+// The row of a 32-row piece that the matrix instruction has as row m: 16 x + 4 a + b -> 16 x + 4 b + a.  Its own inverse.
+__device__ __forceinline__ constexpr int tile_row(int m) { return (m & ~15) | ((m & 3) << 2) | ((m >> 2) & 3); }
 
 // v = p0 + p1 + p2 up to 2^-24 |v|
 __device__ __forceinline__ void split3(float v, BF16& p0, BF16& p1, BF16& p2)
@@ -108,36 +97,43 @@ __device__ __forceinline__ Float16 product(const Bf16x8 (&a)[P], const Bf16x8 (&
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[0], b[0], c, 0, 0, 0);
 }
 
-// Eight columns of a row as they come from memory.
+// Eight columns of a row as they come from memory.  `at` is the first of them, `cols` how many the row has from there on
+// (none, or whole 16-byte pieces); what is not loaded keeps its value.
 template <int P>
 struct RowChunk;
 template <>
 struct RowChunk<1> {
+    static constexpr int kBytes = 16;
     Word4 v;
-    __device__ __forceinline__ void load(const void* base, int64_t row, int64_t stride, int c, int dim)
+    __device__ __forceinline__ void load(const char* at, int cols)
     {
-        v = Word4{0, 0, 0, 0};
-        if (c * 8 < dim) {
-            v = *reinterpret_cast<const Word4*>(static_cast<const BF16*>(base) + row * stride + c * 8);
+        if (cols > 0) {
+            v = *reinterpret_cast<const Word4*>(at);
         }
     }
     __device__ __forceinline__ void clear() { v = Word4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void negate() { v ^= Word4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u}; }
     __device__ __forceinline__ void planes(Bf16x8 (&p)[1]) const { __builtin_memcpy(&p[0], &v, 16); }
 };
 template <>
 struct RowChunk<3> {
+    static constexpr int kBytes = 32;
     Float4 v[2];
-    __device__ __forceinline__ void load(const void* base, int64_t row, int64_t stride, int c, int dim)
+    __device__ __forceinline__ void load(const char* at, int cols)
     {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            v[h] = Float4{0, 0, 0, 0};
-            if (c * 8 + h * 4 < dim) {
-                v[h] = *reinterpret_cast<const Float4*>(static_cast<const float*>(base) + row * stride + c * 8 + h * 4);
-            }
+        if (cols > 0) {
+            v[0] = *reinterpret_cast<const Float4*>(at);
+        }
+        if (cols > 4) {
+            v[1] = *reinterpret_cast<const Float4*>(at + 16);
         }
     }
     __device__ __forceinline__ void clear() { v[0] = v[1] = Float4{0, 0, 0, 0}; }
+    __device__ __forceinline__ void negate()
+    {
+        v[0] = -v[0];
+        v[1] = -v[1];
+    }
     __device__ __forceinline__ void planes(Bf16x8 (&p)[3]) const
     {
 #pragma unroll
@@ -151,6 +147,25 @@ struct RowChunk<3> {
     }
 };
 
+// Columns d .. d + 3 of a row, as far as it has them.
+template <typename T>
+__device__ __forceinline__ void store_columns(T* row, int d, int dim, bool fours, Float4 v)
+{
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    if (fours) {
+        if (d < dim) {
+            *reinterpret_cast<T4*>(row + d) = T4{from_float<T>(v[0]), from_float<T>(v[1]), from_float<T>(v[2]), from_float<T>(v[3])};
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (d + j < dim) {
+                row[d + j] = from_float<T>(v[j]);
+            }
+        }
+    }
+}
+
 // P: planes per operand (1 bfloat16, 3 float32); DP: columns rounded up to 32, 64, 128 or 256; RW: rows a wave owns;
 // OW: owning waves of the block: 4, or fewer: then 4 / OW waves own the same rows and share out the stream's rows.
 template <int P, int DP, int RW, int OW, int PASS>
@@ -163,13 +178,18 @@ struct LossTile {
     // more than what two buffers of LDS and the registers between memory and LDS hold
     static constexpr int kRows = OW < 4 ? 32 * kStreamWaves : (P == 3 && DP > 32) || (DP == 256 && PASS != kLossForward) ? 32 : 64;
     static constexpr int kLoads = kRows * kChunks / kLossThreads;   // chunks per thread and tile
-    static constexpr int kPlane = kRows * DP;                       // elements
-    static constexpr int kBuffers = P * kPlane * 2 * 2 > 131072 ? 1 : 2;
+    static constexpr int kRow = DP + 8;                             // elements from row to row
+    static constexpr int kPlane = kRows * kRow;
+    static constexpr int kBuffers = P * kPlane * 2 * 2 > 147456 ? 1 : 2;
     static_assert(kLoads >= 1 && kLoads * kLossThreads == kRows * kChunks, "whole chunks per thread");
-    static_assert(P * kPlane * 2 * kBuffers <= 131072, "the tiles fit LDS");
+    static_assert(P * kPlane * 2 * kBuffers <= 147456, "the tiles fit LDS");
 };
 
-template <int P, int DP, int RW, int OW, int PASS, int OCC>
+//
+// SHIFT: scores are shifted by a value per item (item_bias, or minus infinity past the end of the table).  A kernel without
+// it takes the last, partial tile with it in a loop of its own: one loop with both forms in it made the compiler move the
+// accumulators from registers to registers in every round.
+template <int P, int DP, int RW, int OW, int PASS, bool SHIFT, int OCC>
 __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
 {
     using L = LossTile<P, DP, RW, OW, PASS>;
@@ -180,9 +200,14 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
     constexpr int CH = L::kChunks;
     constexpr int NB = L::kBuffers;
     __shared__ __attribute__((aligned(16))) BF16 tile[NB][P * L::kPlane];
-    __shared__ __attribute__((aligned(16))) float auxA[NB][TR];                               // forward, dx: bias (base 2); dt: lse (base 2)
-    __shared__ __attribute__((aligned(16))) float auxG[PASS == kLossDt ? NB : 1][PASS == kLossDt ? TR : 1];   // dt: grad * scale
-    __shared__ int32_t auxT[PASS == kLossDt ? NB : 1][PASS == kLossDt ? TR : 1]; // dt: target
+    // per stream row, in the order of the matrix rows: forward, dx: bias (base 2); dt: log2 |grad scale| - lse (base 2)
+    __shared__ __attribute__((aligned(16))) float auxA[NB][TR];
+    constexpr bool kDt = PASS == kLossDt;
+    __shared__ __attribute__((aligned(16))) float auxG[kDt ? NB : 1][kDt ? TR : 1];     // dt: |grad scale|
+    __shared__ __attribute__((aligned(16))) int32_t auxT[kDt ? NB : 1][kDt ? TR : 1];   // dt: target
+    constexpr bool kMasks = SHIFT || kDt;
+    __shared__ uint32_t deadBits[2][kMasks ? TR / 32 : 1];                   // a bit per stream row that takes no part
+    __shared__ uint32_t minusBits[kDt ? NB : 1][kDt ? TR / 32 : 1];          // dt: a bit per row whose grad * scale is negative
 
     const int wave = threadIdx.x / kWave;
     const int lane = lane_id();
@@ -194,9 +219,12 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
     const int streamWave = wave / OW;
     const int tiles = (a.streams + TR - 1) / TR;
     const int t0 = split * a.tilesPerSplit;
-    const int t1 = min(t0 + a.tilesPerSplit, tiles);
-    const float c2 = a.scale * kLog2e;
+    const int t1 = min(t0 + a.tilesPerSplit, tiles);   // t0 < t1: no split is empty
+    // the forward pass bounds scores by the largest product, so there a negative scale goes into the owner's rows
+    const bool turned = PASS == kLossForward && a.scale < 0.0f;
+    const float c2 = (turned ? -a.scale : a.scale) * kLog2e;
     const bool biased = a.bias != nullptr;
+    constexpr int kElement = P == 1 ? 2 : 4;
 
     // ---- the rows this wave owns ----
     Bf16x8 own[CB][KS][P];
@@ -223,71 +251,134 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             RowChunk<P> r;
+            r.clear();   // rows past the end, padding positions and free slots may hold anything
             if (live) {
-                r.load(a.own, n, a.ownStride, ks * 2 + half, a.dim);
-            } else {
-                r.clear();   // rows past the end, padding positions and free slots may hold anything
+                const int c = (ks * 2 + half) * 8;
+                r.load(static_cast<const char*>(a.own) + (n * a.ownStride * kElement + c * kElement), a.dim - c);
+            }
+            if (turned) {
+                r.negate();
             }
             r.planes(own[cb][ks]);
         }
     }
 
     // ---- the stream's tiles: memory -> registers (one tile ahead) -> LDS ----
+    // A thread moves chunk `chunk` of rows chunkRow, chunkRow + kStep, ...: one 32-bit offset per thread for the whole run
+    constexpr int kStep = kLossThreads / CH;
+    const int chunk = threadIdx.x % CH;
+    const int chunkRow = threadIdx.x / CH;
+    const int chunkCols = a.dim - chunk * 8;
+    const int64_t strideBytes = a.streamStride * kElement;
+    const uint32_t chunkAt = (uint32_t)(chunkRow * strideBytes + chunk * RowChunk<P>::kBytes);
     RowChunk<P> staged[L::kLoads];
-    float stagedA = 0.0f;
-    float stagedG = 0.0f;
-    int32_t stagedT = -1;
-    bool stagedLive[L::kLoads];
-    auto fetch = [&](int t) {
 #pragma unroll
-        for (int q = 0; q < L::kLoads; ++q) {
-            const int i = q * kLossThreads + threadIdx.x;
-            const int64_t row = (int64_t)t * TR + i / CH;
-            const int64_t at = row < a.streams ? row : a.streams - 1;
-            bool live = row < a.streams;
-            if constexpr (PASS == kLossDt) {
-                live = live && a.lse[at] != INFINITY;
-            } else if (biased) {
-                live = live && a.bias[at] > kMaskedBelow;
+    for (int q = 0; q < L::kLoads; ++q) {
+        staged[q].clear();
+    }
+    auto fetch = [&](int t) {
+        const char* base = static_cast<const char*>(a.stream) + (int64_t)t * TR * strideBytes;
+        if ((t + 1) * (int64_t)TR <= a.streams) {
+#pragma unroll
+            for (int q = 0; q < L::kLoads; ++q) {
+                staged[q].load(base + q * kStep * strideBytes + chunkAt, chunkCols);
             }
-            stagedLive[q] = live;
-            staged[q].load(a.stream, at, a.streamStride, i % CH, a.dim);
-        }
-        if (threadIdx.x < TR) {
-            const int64_t row = (int64_t)t * TR + threadIdx.x;
-            if constexpr (PASS == kLossDt) {
-                const float l = row < a.streams ? a.lse[row] : INFINITY;
-                const bool live = l != INFINITY;   // a NaN stays one
-                stagedA = live ? l * kLog2e : INFINITY;
-                stagedG = live ? a.grad[row] * a.scale : 0.0f;
-                stagedT = live ? (int32_t)a.target[row] : -1;
-            } else {
-                const float b = row >= a.streams ? -INFINITY : biased ? a.bias[row] : 0.0f;
-                stagedA = b > kMaskedBelow ? b * kLog2e : -INFINITY;
+        } else {   // rows past the end: the last one instead
+            const int last = a.streams - 1 - t * TR;
+#pragma unroll
+            for (int q = 0; q < L::kLoads; ++q) {
+                const int r = min(q * kStep + chunkRow, last);
+                staged[q].load(base + (int64_t)r * strideBytes + chunk * RowChunk<P>::kBytes, chunkCols);
             }
         }
     };
-    auto place = [&](int buf) {
+    // What goes with a stream row: one thread per row, two tiles ahead, so that by the time a tile is placed it is known
+    // which of its rows take no part and have to be zero (0 times whatever lies there must be 0).
+    struct Aux {
+        float a;
+        float g;
+        int32_t t;
+        bool dead;
+        bool minus;
+    };
+    auto aux_load = [&](int t) {
+        Aux x = {-INFINITY, 0.0f, -1, true, false};
+        if constexpr (kMasks) {
+            const int64_t row = (int64_t)t * TR + threadIdx.x;
+            if (threadIdx.x < TR && t < t1 && row < a.streams) {
+                if constexpr (kDt) {
+                    const float l = a.lse[row];
+                    x.dead = l == INFINITY;   // a NaN stays one
+                    if (!x.dead) {
+                        const float g = a.grad[row] * a.scale;
+                        x.g = fabsf(g);
+                        x.minus = g < 0.0f;
+                        x.a = log2f(x.g) - l * kLog2e;
+                        x.t = (int32_t)a.target[row];
+                    }
+                } else {
+                    const float b = a.bias == nullptr ? 0.0f : a.bias[row];
+                    x.dead = b <= kMaskedBelow;
+                    x.a = x.dead ? -INFINITY : b * kLog2e;
+                }
+            }
+        }
+        return x;
+    };
+    auto aux_mark = [&](const Aux& x, int t) {
+        if constexpr (kMasks) {
+            const unsigned long long dead = __ballot(x.dead);
+            if (threadIdx.x < TR && (lane & 31) == 0) {
+                deadBits[t & 1][threadIdx.x / 32] = (uint32_t)(dead >> (lane & 32));
+            }
+        }
+    };
+    auto place = [&](int buf, int t, const Aux& x) {
+        if constexpr (kMasks) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int w = 0; w < TR / 32; ++w) {
+                any |= deadBits[t & 1][w];
+            }
+            if (__builtin_amdgcn_readfirstlane(any) != 0) {
+#pragma unroll
+                for (int q = 0; q < L::kLoads; ++q) {
+                    const int r = q * kStep + chunkRow;
+                    if ((deadBits[t & 1][r / 32] >> (r % 32)) & 1) {
+                        staged[q].clear();
+                    }
+                }
+            }
+            const unsigned long long minus = __ballot(x.minus);
+            if (threadIdx.x < TR) {
+                const int at = (threadIdx.x & ~31) | tile_row(threadIdx.x & 31);
+                auxA[buf][at] = x.a;
+                if constexpr (kDt) {
+                    auxG[buf][at] = x.g;
+                    auxT[buf][at] = x.t;
+                    if ((lane & 31) == 0) {
+                        minusBits[buf][threadIdx.x / 32] = (uint32_t)(minus >> (lane & 32));
+                    }
+                }
+            }
+        } else if ((t + 1) * (int64_t)TR > a.streams) {
+#pragma unroll
+            for (int q = 0; q < L::kLoads; ++q) {
+                if (t * TR + q * kStep + chunkRow >= a.streams) {
+                    staged[q].clear();
+                }
+            }
+            if (threadIdx.x < TR) {
+                auxA[buf][(threadIdx.x & ~31) | tile_row(threadIdx.x & 31)] = t * TR + (int)threadIdx.x < a.streams ? 0.0f : -INFINITY;
+            }
+        }
 #pragma unroll
         for (int q = 0; q < L::kLoads; ++q) {
-            const int i = q * kLossThreads + threadIdx.x;
-            const int r = i / CH;
-            const int c = swizzle<CH>(r, i % CH);
-            if (!stagedLive[q]) {
-                staged[q].clear();   // 0 times whatever lies there must be 0
-            }
             Bf16x8 p[P];
             staged[q].planes(p);
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                *reinterpret_cast<Bf16x8*>(&tile[buf][k * L::kPlane + r * DP + c * 8]) = p[k];
-            }
-        }
-        if (threadIdx.x < TR) {
-            auxA[buf][threadIdx.x] = stagedA;
-            if constexpr (PASS == kLossDt) {
-                auxG[buf][threadIdx.x] = stagedG;
-                auxT[buf][threadIdx.x] = stagedT;
+                *reinterpret_cast<Bf16x8*>(&tile[buf][k * L::kPlane + (q * kStep + chunkRow) * L::kRow + chunk * 8]) = p[k];
             }
         }
     };
@@ -313,7 +404,7 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
     // ---- one 32-row piece of a tile ----
     auto piece = [&](auto shiftedC, int buf, int r0, int rowBase) {
         constexpr bool shifted = decltype(shiftedC)::value;
-        const BF16* base = tile[buf];
+        const BF16* rowAt = &tile[buf][(r0 + tile_row(col)) * L::kRow + half * 8];
         Float16 s[CB];
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
@@ -325,20 +416,19 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
             Bf16x8 x[P];
-            const int r = r0 + col;
-            const int c = swizzle<CH>(r, ks * 2 + half);
 #pragma unroll
             for (int k = 0; k < P; ++k) {
-                x[k] = *reinterpret_cast<const Bf16x8*>(base + k * L::kPlane + r * DP + c * 8);
+                x[k] = *reinterpret_cast<const Bf16x8*>(rowAt + k * L::kPlane + ks * 16);
             }
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
                 s[cb] = product<P>(x, own[cb][ks], s[cb]);
             }
         }
-        // register i of a lane holds stream row r0 + 8 (i / 4) + 4 half + i % 4, owner row ownBase + cb * 32 + col
+        // register i of a lane holds matrix row 8 (i / 4) + 4 half + i % 4, owner row ownBase + cb * 32 + col
         if constexpr (PASS == kLossForward) {
             float b[16];
+            float most = 0.0f;   // largest shift
             if constexpr (shifted) {
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -348,25 +438,34 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
                         b[4 * q + j] = v[j];
                     }
                 }
+                most = b[0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) {
+                    most = fmaxf(most, b[i]);
+                }
             }
 #pragma unroll
             for (int cb = 0; cb < CB; ++cb) {
-                float most = -INFINITY;
+                // The maximum follows only when it has fallen behind by 2^kSlack (the sums have room for that), so what is
+                // asked of every score is a bound: the largest product (c2 is not negative) plus the largest shift.
+                float high = s[cb][0];
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    s[cb][i] = shifted ? __builtin_fmaf(s[cb][i], c2, b[i]) : s[cb][i] * c2;
-                    most = fmaxf(most, s[cb][i]);
+                for (int i = 1; i < 16; ++i) {
+                    high = fmaxf(high, s[cb][i]);
                 }
-                // the maximum follows only when it has fallen far behind: sums up to 2^kSlack per item fit easily
-                if (__any(most > top[cb] + kSlack)) {
-                    const float now = fmaxf(top[cb], most);
+                if (__any(__builtin_fmaf(high, c2, most) > top[cb] + kSlack)) {
+                    float now = top[cb];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        now = fmaxf(now, shifted ? __builtin_fmaf(s[cb][i], c2, b[i]) : s[cb][i] * c2);
+                    }
                     sum[cb] *= exp2_fast(top[cb] - now);
                     top[cb] = now;
                 }
                 float add = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    add += exp2_fast(s[cb][i] - top[cb]);
+                    add += exp2_fast(__builtin_fmaf(s[cb][i], c2, shifted ? b[i] - top[cb] : -top[cb]));
                 }
                 sum[cb] += add;
             }
@@ -391,29 +490,29 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
                     for (int i = 0; i < 16; ++i) {
                         s[cb][i] = exp2_fast(__builtin_fmaf(s[cb][i], c2, shifted ? b[i] + shift : shift));
                     }
-                    const int d = ownTarget[cb] - rowBase;
-                    if (__any(d >= 0 && d < 32)) {
+                    int d = ownTarget[cb] - rowBase;
+                    if (__any((unsigned)d < 32u)) {
+                        d -= half;   // tile_row of a matrix row with 4 half in it
+                        pin(d);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            s[cb][i] -= d == 8 * (i / 4) + 4 * half + i % 4 ? 1.0f : 0.0f;
+                            s[cb][i] -= d == tile_row(8 * (i / 4) + i % 4) ? 1.0f : 0.0f;
                         }
                     }
                 }
             } else {
+                // |grad scale| is in the exponent; its sign, and the 1 at the target, are rarely asked for
                 float shift[16];
-                float gr[16];
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     const Float4 v = *reinterpret_cast<const Float4*>(&auxA[buf][r0 + 8 * q + 4 * half]);
-                    const Float4 w = *reinterpret_cast<const Float4*>(&auxG[buf][r0 + 8 * q + 4 * half]);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        shift[4 * q + j] = -v[j];
-                        gr[4 * q + j] = w[j];
+                        shift[4 * q + j] = v[j];
                     }
                 }
-                const int mine = auxT[buf][r0 + col] - ownBase;
-                const bool hit = __any(mine >= 0 && mine < RW);
+                const bool hit = __any((unsigned)(auxT[buf][r0 + col] - ownBase) < (unsigned)RW);
+                const uint32_t minus = __builtin_amdgcn_readfirstlane(minusBits[buf][r0 / 32]);
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
 #pragma unroll
@@ -421,15 +520,19 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
                         s[cb][i] = exp2_fast(__builtin_fmaf(s[cb][i], c2, shifted ? shift[i] + ownShift[cb] : shift[i]));
                     }
                     if (hit) {
+                        int mine = ownBase + cb * 32 + col;
+                        pin(mine);
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
-                            const int d = auxT[buf][r0 + 8 * (i / 4) + 4 * half + i % 4] - ownBase;
-                            s[cb][i] -= d == cb * 32 + col ? 1.0f : 0.0f;
+                            const int m = r0 + 8 * (i / 4) + 4 * half + i % 4;
+                            s[cb][i] -= auxT[buf][m] == mine ? auxG[buf][m] : 0.0f;
                         }
                     }
+                    if (minus != 0) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        s[cb][i] *= gr[i];
+                        for (int i = 0; i < 16; ++i) {
+                            s[cb][i] = ((minus >> tile_row(8 * (i / 4) + i % 4)) >> half) & 1 ? -s[cb][i] : s[cb][i];
+                        }
                     }
                 }
             }
@@ -449,7 +552,7 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
                 }
             }
             // second product: contracted over the piece's rows, in the order in which the registers hold them
-            const int quad = (lane & 15) >> 2;
+            const BF16* columnAt = &tile[buf][(r0 + 4 * ((lane & 15) >> 2) + half) * L::kRow + ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
 #pragma unroll
             for (int db = 0; db < DB; ++db) {
 #pragma unroll
@@ -460,9 +563,7 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
                         Short4 v[2];
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
-                            const int r = r0 + 16 * kk + 8 * j + 4 * half + quad;
-                            const int c = swizzle<CH>(r, db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1));
-                            const BF16* p = base + k * L::kPlane + r * DP + c * 8 + (lane & 1) * 4;
+                            const BF16* p = columnAt + k * L::kPlane + (16 * kk + 2 * j) * L::kRow + db * 32;
                             v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                 (__attribute__((address_space(3))) Short4*)(const_cast<BF16*>(p)));
                         }
@@ -470,51 +571,58 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
                     }
 #pragma unroll
                     for (int cb = 0; cb < CB; ++cb) {
-                        acc[cb][db] = product<P>(g[cb][kk], w, acc[cb][db]);
+                        acc[cb][db] = product<P>(w, g[cb][kk], acc[cb][db]);
                     }
                 }
             }
         }
     };
 
-    auto compute = [&](int buf, int t) {
-        const int rows = min(TR, a.streams - t * TR);
-        if (biased || (PASS != kLossDt && rows < TR)) {
+    Aux next = aux_load(t0);   // of the tile that is placed next
+    auto sweep = [&](auto shiftedC, int from, int to) {
 #pragma unroll 1
-            for (int r0 = streamWave * 32; r0 < rows; r0 += 32 * L::kStreamWaves) {
-                piece(Yes{}, buf, r0, t * TR + r0);
-            }
-        } else {
-#pragma unroll 1
-            for (int r0 = streamWave * 32; r0 < rows; r0 += 32 * L::kStreamWaves) {
-                piece(No{}, buf, r0, t * TR + r0);
-            }
-        }
-    };
-
-    const bool idle = ownBase >= a.owners;   // the wave owns nothing, but keeps the barriers and moves its share
-    if (t0 < t1) {
-        fetch(t0);
-        place(0);
-        __syncthreads();
-        for (int t = t0; t < t1; ++t) {
+        for (int t = from; t < to; ++t) {
             const int buf = NB == 2 ? (t - t0) & 1 : 0;
-            if (t + 1 < t1) {
+            const bool more = t + 1 < t1;
+            if (more) {
                 fetch(t + 1);
             }
-            if (!idle) {
-                compute(buf, t);
+            const Aux after = aux_load(t + 2);
+            // no condition around the pieces: a wave without rows of its own, or rows past the stream's end, compute zeros
+#pragma unroll 1
+            for (int k = 0; k < TR / 32 / L::kStreamWaves; ++k) {
+                const int r0 = (k * L::kStreamWaves + streamWave) * 32;
+                piece(shiftedC, buf, r0, t * TR + r0);
             }
             if (NB == 1) {
                 __syncthreads();
             }
-            if (t + 1 < t1) {
-                place(NB == 2 ? buf ^ 1 : 0);
+            if (more) {
+                place(NB == 2 ? buf ^ 1 : 0, t + 1, next);
             }
+            aux_mark(after, t + 2);
+            next = after;
             __syncthreads();
         }
+    };
+    if (t0 < t1) {
+        fetch(t0);
+        aux_mark(next, t0);
+        const Aux second = aux_load(t0 + 1);
+        aux_mark(second, t0 + 1);
+        __syncthreads();
+        place(0, t0, next);
+        next = second;
+        __syncthreads();
+        if constexpr (SHIFT || kDt) {
+            sweep(std::integral_constant<bool, SHIFT>{}, t0, t1);
+        } else {
+            const int whole = max(t0, min(t1, a.streams / TR));
+            sweep(std::false_type{}, t0, whole);
+            sweep(std::true_type{}, whole, t1);
+        }
     }
-    if (idle) {
+    if (ownBase >= a.owners) {
         return;
     }
 
@@ -532,23 +640,24 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
             }
         }
     } else {
+        const bool fours = a.dim % 4 == 0;   // then every group of four columns is whole and aligned
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
+            const int n = ownBase + cb * 32 + col;
+            if (n >= a.owners) {
+                continue;
+            }
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int n = ownBase + cb * 32 + 8 * (i / 4) + 4 * half + i % 4;
-#pragma unroll
-                for (int db = 0; db < DB; ++db) {
-                    const int d = db * 32 + col;
-                    if (n < a.owners && d < a.dim) {
-                        if (a.part != nullptr) {
-                            a.part[(partRow + n) * a.dim + d] = acc[cb][db][i];
-                        } else if constexpr (P == 1) {
-                            static_cast<BF16*>(a.out)[(int64_t)n * a.dim + d] = (BF16)acc[cb][db][i];
-                        } else {
-                            static_cast<float*>(a.out)[(int64_t)n * a.dim + d] = acc[cb][db][i];
-                        }
-                    }
+            for (int q = 0; q < DB * 4; ++q) {
+                const int d = q * 8 + 4 * half;
+                const Float4 v = {acc[cb][q / 4][q % 4 * 4], acc[cb][q / 4][q % 4 * 4 + 1], acc[cb][q / 4][q % 4 * 4 + 2],
+                                  acc[cb][q / 4][q % 4 * 4 + 3]};
+                if (a.part != nullptr) {
+                    store_columns(a.part + (partRow + n) * a.dim, d, a.dim, fours, v);
+                } else if constexpr (P == 1) {
+                    store_columns(static_cast<BF16*>(a.out) + (int64_t)n * a.dim, d, a.dim, fours, v);
+                } else {
+                    store_columns(static_cast<float*>(a.out) + (int64_t)n * a.dim, d, a.dim, fours, v);
                 }
             }
         }
@@ -612,26 +721,55 @@ __global__ __launch_bounds__(kBlock) void k_softmax_loss_join(const float2* __re
     }
 }
 
-// out = factor(row) * sum of the parts, in their order, in the operands' type.
-template <typename T>
+// out = factor(row) * sum of the parts, in the operands' type.  Four neighbouring values per thread (E = 4 where rows are
+// whole fours); the WAYS thread groups of a block take every WAYS-th part each and are joined in their order, so that few
+// values with many parts (few rows against a long table) still have many loads in flight.
+template <typename T, int E, int WAYS>
 __global__ __launch_bounds__(kBlock) void k_softmax_grad_join(const float* __restrict__ part, int parts, int64_t count, int dim,
                                                               const float* __restrict__ lse, const float* __restrict__ grad,
                                                               float scale, T* __restrict__ out)
 {
-    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    constexpr int kWide = kBlock / WAYS;
+    typedef float FloatE __attribute__((ext_vector_type(E)));
+    typedef T OutE __attribute__((ext_vector_type(E)));
+    __shared__ FloatE sums[WAYS > 1 ? WAYS : 1][WAYS > 1 ? kWide : 1];
+    const int way = threadIdx.x / kWide;
+    const int at = threadIdx.x % kWide;
+    const int64_t i = ((int64_t)blockIdx.x * kWide + at) * E;
+    FloatE s = 0.0f;
+    if (i < count) {
+#pragma unroll 8
+        for (int p = way; p < parts; p += WAYS) {
+            s += *reinterpret_cast<const FloatE*>(part + p * count + i);
+        }
+    }
+    if constexpr (WAYS > 1) {
+        sums[way][at] = s;
+        __syncthreads();
+        if (way != 0) {
+            return;
+        }
+#pragma unroll
+        for (int w = 1; w < WAYS; ++w) {
+            s += sums[w][at];
+        }
+    }
     if (i >= count) {
         return;
     }
-    float s = 0.0f;
-#pragma unroll 8
-    for (int p = 0; p < parts; ++p) {
-        s += part[p * count + i];
-    }
+    float factor = 1.0f;
+    bool live = true;
     if (grad != nullptr) {
         const int64_t n = i / dim;
-        s = lse[n] != INFINITY ? s * (grad[n] * scale) : 0.0f;
+        live = lse[n] != INFINITY;
+        factor = grad[n] * scale;
     }
-    out[i] = from_float<T>(s);
+    OutE o;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        o[e] = from_float<T>(live ? s[e] * factor : 0.0f);
+    }
+    *reinterpret_cast<OutE*>(out + i) = o;
 }
 
 // Rows of `dim` elements at any stride -> rows of `padded` elements, the rest zero.
@@ -664,6 +802,13 @@ struct PassPlan {
 
 static int padded_dim(int dim) { return dim <= 32 ? 32 : dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
+// Rows a wave owns where there are many: 64 (every LDS read feeds two matrix instructions) while two waves per SIMD fit the
+// registers, else 32; two waves matter more (128 columns, 2048 x 1 M, dx: 1.17 ms with 32 rows, 1.27 with 64 and one wave).
+static constexpr int wide_rows(int planes, int dp, int pass)
+{
+    return planes == 1 && (dp < 128 || pass == kLossForward) ? 64 : 32;
+}
+
 static int tile_rows(int planes, int dp, int ownWaves, int pass)
 {
     return ownWaves < 4 ? 32 * (4 / ownWaves) : (planes == 3 && dp > 32) || (dp == 256 && pass != kLossForward) ? 32 : 64;
@@ -673,7 +818,7 @@ static PassPlan plan_pass(int planes, int dim, int64_t owners, int64_t streams, 
 {
     const int dp = padded_dim(dim);
     PassPlan p{};
-    p.rowsPerWave = planes == 3 || (dp == 256 && pass != kLossForward) ? 32 : 64;
+    p.rowsPerWave = wide_rows(planes, dp, pass);
     p.ownWaves = 4;
     if (pass != kLossDt) {
         if (owners <= 128) {
@@ -731,36 +876,34 @@ static LossPlan plan_loss(int64_t rows, int64_t items, int32_t dim, int32_t dtyp
     return p;
 }
 
-template <int P, int DP, int RW, int OW, int PASS, int OCC>
+template <int P, int DP, int RW, int OW, int PASS, bool SHIFT, int OCC>
 static int launch_tiles(const LossArgs& a, const PassPlan& p, hipStream_t stream)
 {
     const char* name = PASS == kLossForward ? "k_softmax_forward" : PASS == kLossDx ? "k_softmax_dx" : "k_softmax_dt";
-    RECSDK_LAUNCH_AS(name, (k_softmax_tiles<P, DP, RW, OW, PASS, OCC>), dim3((unsigned)(p.blocks * p.splits)), dim3(kLossThreads),
-                     stream, a);
+    RECSDK_LAUNCH_AS(name, (k_softmax_tiles<P, DP, RW, OW, PASS, SHIFT, OCC>), dim3((unsigned)(p.blocks * p.splits)),
+                     dim3(kLossThreads), stream, a);
     return RECSDK_OK;
 }
 
 template <int P, int DP, int PASS>
 static int launch_width(const LossArgs& a, const PassPlan& p, hipStream_t stream)
 {
-    constexpr int kOcc = P == 3 && DP == 256 ? 1 : 2;
+    constexpr int kOcc = PASS == kLossForward ? (DP == 256 ? 1 : 2) : (P == 3 && DP == 256) ? 1 : 2;
+    constexpr int kWide = wide_rows(P, DP, PASS);
     if constexpr (PASS != kLossDt) {
         constexpr int kNarrow = P == 3 && DP == 256 ? 2 : 1;
         if (p.ownWaves == kNarrow) {
-            constexpr int kNarrowOcc = DP == 256 || (P == 3 && DP == 128) ? 1 : 2;
-            return launch_tiles<P, DP, 32, kNarrow, PASS, kNarrowOcc>(a, p, stream);
+            constexpr int kNarrowOcc = DP >= 128 || (P == 3 && DP == 64) ? 1 : 2;
+            return launch_tiles<P, DP, 32, kNarrow, PASS, true, kNarrowOcc>(a, p, stream);
+        }
+        if constexpr (kWide == 64) {
+            if (p.rowsPerWave == 32) {
+                return launch_tiles<P, DP, 32, 4, PASS, true, 2>(a, p, stream);
+            }
         }
     }
-    if constexpr (P == 1 && (DP < 256 || PASS == kLossForward)) {
-        if (p.rowsPerWave == 64) {
-            return launch_tiles<P, DP, 64, 4, PASS, kOcc>(a, p, stream);
-        }
-    }
-    if constexpr (PASS != kLossDt || P == 3 || DP == 256) {
-        return launch_tiles<P, DP, 32, 4, PASS, kOcc>(a, p, stream);
-    }
-    set_error("softmax loss: no kernel for this shape");
-    return RECSDK_EINVAL;
+    return a.bias != nullptr ? launch_tiles<P, DP, kWide, 4, PASS, true, kOcc>(a, p, stream)
+                             : launch_tiles<P, DP, kWide, 4, PASS, false, kOcc>(a, p, stream);
 }
 
 template <int PASS>
@@ -812,6 +955,10 @@ static int check_loss(const char* name, int64_t rows, int64_t items, int32_t dim
         set_error("%s: rows overlap (stride < dim)", name);
         return RECSDK_EINVAL;
     }
+    if (x_stride > kLossMaxStride || table_stride > kLossMaxStride) {
+        set_error("%s: rows are more than %d elements apart", name, kLossMaxStride);
+        return RECSDK_EINVAL;
+    }
     return RECSDK_OK;
 }
 
@@ -826,6 +973,32 @@ static int pad_operand(const void*& p, int64_t& stride, int64_t rows, int dim, i
     p = to;
     stride = padded;
     return RECSDK_OK;
+}
+
+template <typename T, int E, int WAYS>
+static int launch_grad_join(const float* part, int parts, int64_t count, int dim, const float* lse, const float* grad,
+                            float scale, T* out, hipStream_t stream)
+{
+    const int64_t grid = cdiv(count, (int64_t)kBlock / WAYS * E);
+    RECSDK_REQUIRE(grid < (int64_t(1) << 31), RECSDK_EINVAL, "softmax loss: table too large for one launch");
+    RECSDK_LAUNCH_AS("k_softmax_grad_join", (k_softmax_grad_join<T, E, WAYS>), dim3((unsigned)grid), dim3(kBlock), stream, part,
+                     parts, count, dim, lse, grad, scale, out);
+    return RECSDK_OK;
+}
+
+template <typename T>
+static int join_grad(const float* part, int parts, int64_t count, int dim, const float* lse, const float* grad, float scale,
+                     void* out, hipStream_t stream)
+{
+    T* o = static_cast<T*>(out);
+    const bool fours = dim % 4 == 0;
+    // 16 ways where there are parts for all of them
+    if (parts >= 16) {
+        return fours ? launch_grad_join<T, 4, 16>(part, parts, count, dim, lse, grad, scale, o, stream)
+                     : launch_grad_join<T, 1, 16>(part, parts, count, dim, lse, grad, scale, o, stream);
+    }
+    return fours ? launch_grad_join<T, 4, 1>(part, parts, count, dim, lse, grad, scale, o, stream)
+                 : launch_grad_join<T, 1, 1>(part, parts, count, dim, lse, grad, scale, o, stream);
 }
 
 struct LossOperands {
@@ -911,8 +1084,10 @@ static int run_backward(const LossPlan& plan, LossOperands o, int64_t rows, int6
         if (rc != RECSDK_OK) {
             return rc;
         }
-        RECSDK_LAUNCH_AS("k_softmax_grad_join", (k_softmax_grad_join<T>), dim3((unsigned)cdiv(rows * dim, kBlock)), dim3(kBlock),
-                         stream, part, plan.dx.parts, rows * dim, dim, lse, grad, scale, static_cast<T*>(dx));
+        rc = join_grad<T>(part, plan.dx.parts, rows * dim, dim, lse, grad, scale, dx, stream);
+        if (rc != RECSDK_OK) {
+            return rc;
+        }
     }
     if (dtable != nullptr) {
         a.own = o.table;
@@ -928,9 +1103,7 @@ static int run_backward(const LossPlan& plan, LossOperands o, int64_t rows, int6
             return rc;
         }
         if (a.part != nullptr) {
-            RECSDK_LAUNCH_AS("k_softmax_grad_join", (k_softmax_grad_join<T>), dim3((unsigned)cdiv(items * dim, kBlock)),
-                             dim3(kBlock), stream, part, plan.dt.parts, items * dim, dim, nullptr, nullptr, scale,
-                             static_cast<T*>(dtable));
+            return join_grad<T>(part, plan.dt.parts, items * dim, dim, nullptr, nullptr, scale, dtable, stream);
         }
     }
     return RECSDK_OK;
@@ -1002,23 +1175,17 @@ extern "C" int recsdk_softmax_loss_backward(const float* d_grad_loss, const void
     hipStream_t s = static_cast<hipStream_t>(stream);
     if (rows == 0) {
         if (d_dtable != nullptr) {
-            const int64_t n = items * dim;
-            RECSDK_REQUIRE(cdiv(n, kBlock) < (int64_t(1) << 31), RECSDK_EINVAL,
-                           "recsdk_softmax_loss_backward: table too large for one launch");
-            if (dtype == RECSDK_DT_F32) {
-                RECSDK_LAUNCH_AS("k_softmax_grad_join", (k_softmax_grad_join<float>), dim3((unsigned)cdiv(n, kBlock)), dim3(kBlock),
-                                 s, nullptr, 0, n, dim, nullptr, nullptr, scale, static_cast<float*>(d_dtable));
-            } else {
-                RECSDK_LAUNCH_AS("k_softmax_grad_join", (k_softmax_grad_join<BF16>), dim3((unsigned)cdiv(n, kBlock)), dim3(kBlock),
-                                 s, nullptr, 0, n, dim, nullptr, nullptr, scale, static_cast<BF16*>(d_dtable));
-            }
+            RECSDK_REQUIRE(aligned16(d_dtable), RECSDK_EINVAL, "recsdk_softmax_loss_backward: dtable must be 16-byte aligned");
+            return dtype == RECSDK_DT_F32
+                       ? join_grad<float>(nullptr, 0, items * dim, dim, nullptr, nullptr, scale, d_dtable, s)
+                       : join_grad<BF16>(nullptr, 0, items * dim, dim, nullptr, nullptr, scale, d_dtable, s);
         }
         return RECSDK_OK;
     }
     RECSDK_REQUIRE(d_grad_loss != nullptr && d_x != nullptr && d_table != nullptr && d_target != nullptr && d_lse != nullptr,
                    RECSDK_ENULL, "recsdk_softmax_loss_backward: NULL argument");
-    RECSDK_REQUIRE(aligned16(d_x) && aligned16(d_table) && aligned16(d_workspace), RECSDK_EINVAL,
-                   "recsdk_softmax_loss_backward: x, table and workspace must be 16-byte aligned");
+    RECSDK_REQUIRE(aligned16(d_x) && aligned16(d_table) && aligned16(d_workspace) && aligned16(d_dx) && aligned16(d_dtable),
+                   RECSDK_EINVAL, "recsdk_softmax_loss_backward: x, table, dx, dtable and workspace must be 16-byte aligned");
     const LossPlan p = plan_loss(rows, items, dim, dtype, x_stride, table_stride);
     RECSDK_REQUIRE(d_workspace != nullptr && workspace_bytes >= p.backwardBytes, RECSDK_ECAPACITY,
                    "recsdk_softmax_loss_backward: the workspace is smaller than recsdk_softmax_loss_workspace says");
