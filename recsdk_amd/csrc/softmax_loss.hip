@@ -294,39 +294,44 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
     };
     // What goes with a stream row: one thread per row, two tiles ahead, so that by the time a tile is placed it is known
     // which of its rows take no part and have to be zero (0 times whatever lies there must be 0).
+    // The loads are issued ahead of the compute and looked at behind it (aux_mark).
     struct Aux {
         float a;
         float g;
-        int32_t t;
+        int64_t t;
         bool dead;
         bool minus;
     };
     auto aux_load = [&](int t) {
-        Aux x = {-INFINITY, 0.0f, -1, true, false};
+        Aux x = {0.0f, 0.0f, -1, true, false};
         if constexpr (kMasks) {
             const int64_t row = (int64_t)t * TR + threadIdx.x;
             if (threadIdx.x < TR && t < t1 && row < a.streams) {
+                x.dead = false;
                 if constexpr (kDt) {
-                    const float l = a.lse[row];
-                    x.dead = l == INFINITY;   // a NaN stays one
-                    if (!x.dead) {
-                        const float g = a.grad[row] * a.scale;
-                        x.g = fabsf(g);
-                        x.minus = g < 0.0f;
-                        x.a = log2f(x.g) - l * kLog2e;
-                        x.t = (int32_t)a.target[row];
-                    }
-                } else {
-                    const float b = a.bias == nullptr ? 0.0f : a.bias[row];
-                    x.dead = b <= kMaskedBelow;
-                    x.a = x.dead ? -INFINITY : b * kLog2e;
+                    x.a = a.lse[row];
+                    x.g = a.grad[row];
+                    x.t = a.target[row];
+                } else if (biased) {
+                    x.a = a.bias[row];
                 }
             }
         }
         return x;
     };
-    auto aux_mark = [&](const Aux& x, int t) {
+    auto aux_mark = [&](Aux& x, int t) {
         if constexpr (kMasks) {
+            if constexpr (kDt) {
+                x.dead = x.dead || x.a == INFINITY;   // a NaN stays one
+                const float g = x.dead ? 0.0f : x.g * a.scale;
+                x.minus = g < 0.0f;
+                x.g = fabsf(g);
+                x.a = x.dead ? -INFINITY : log2f(x.g) - x.a * kLog2e;
+                x.t = x.dead ? -1 : x.t;
+            } else {
+                x.dead = x.dead || x.a <= kMaskedBelow;
+                x.a = x.dead ? -INFINITY : x.a * kLog2e;
+            }
             const unsigned long long dead = __ballot(x.dead);
             if (threadIdx.x < TR && (lane & 31) == 0) {
                 deadBits[t & 1][threadIdx.x / 32] = (uint32_t)(dead >> (lane & 32));
@@ -355,7 +360,7 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
                 auxA[buf][at] = x.a;
                 if constexpr (kDt) {
                     auxG[buf][at] = x.g;
-                    auxT[buf][at] = x.t;
+                    auxT[buf][at] = (int32_t)x.t;
                     if ((lane & 31) == 0) {
                         minusBits[buf][threadIdx.x / 32] = (uint32_t)(minus >> (lane & 32));
                     }
@@ -584,10 +589,10 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
         for (int t = from; t < to; ++t) {
             const int buf = NB == 2 ? (t - t0) & 1 : 0;
             const bool more = t + 1 < t1;
+            Aux after = aux_load(t + 2);
             if (more) {
                 fetch(t + 1);
             }
-            const Aux after = aux_load(t + 2);
             // no condition around the pieces: a wave without rows of its own, or rows past the stream's end, compute zeros
 #pragma unroll 1
             for (int k = 0; k < TR / 32 / L::kStreamWaves; ++k) {
@@ -606,9 +611,9 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
         }
     };
     if (t0 < t1) {
+        Aux second = aux_load(t0 + 1);
         fetch(t0);
         aux_mark(next, t0);
-        const Aux second = aux_load(t0 + 1);
         aux_mark(second, t0 + 1);
         __syncthreads();
         place(0, t0, next);
@@ -787,7 +792,15 @@ __global__ __launch_bounds__(kBlock) void k_pad_rows(const T* __restrict__ src, 
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
-constexpr int kLossResident = 512;   // blocks the card holds at once (two per compute unit)
+// Blocks that a compute unit holds at once, by the registers and LDS of the tile kernels.
+static int resident_blocks(int planes, int dp, int pass)
+{
+    if (pass == kLossForward) {
+        return planes == 1 ? (dp <= 64 ? 4 : dp == 128 ? 3 : 1) : dp == 32 ? 4 : dp == 64 ? 3 : dp == 128 ? 2 : 1;
+    }
+    return planes == 1 ? (dp == 32 ? 3 : 2) : dp == 32 ? 4 : dp <= 128 ? 2 : 1;
+}
+constexpr int kComputeUnits = 256;
 
 // What one pass launches.
 struct PassPlan {
@@ -832,7 +845,7 @@ static PassPlan plan_pass(int planes, int dim, int64_t owners, int64_t streams, 
     p.tileRows = tile_rows(planes, dp, p.ownWaves, pass);
     p.blocks = cdiv(owners, (int64_t)p.rowsPerWave * p.ownWaves);
     const int64_t tiles = cdiv(streams, p.tileRows);
-    int64_t splits = kLossResident / p.blocks;
+    int64_t splits = (int64_t)kComputeUnits * resident_blocks(planes, dp, pass) / p.blocks;
     splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
     p.tilesPerSplit = (int)cdiv(tiles, splits);
     p.splits = (int)cdiv(tiles, p.tilesPerSplit);
