@@ -61,7 +61,8 @@ struct LossArgs {
     int32_t splits;         // pieces of the stream
     int32_t tilesPerSplit;
     float2* norm;           // forward: [split parts][owners] (maximum, sum), base 2
-    float* part;            // backward: [split parts][owners][dim] partial sums, or NULL
+    float* part;            // backward: [split parts][owners][partDim] partial sums, or NULL
+    int32_t partDim;        // dim rounded up to whole fours
     void* out;              // dt pass without parts: [owners][dim] in the operands' type
 };
 
@@ -658,7 +659,7 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
                 const Float4 v = {acc[cb][q / 4][q % 4 * 4], acc[cb][q / 4][q % 4 * 4 + 1], acc[cb][q / 4][q % 4 * 4 + 2],
                                   acc[cb][q / 4][q % 4 * 4 + 3]};
                 if (a.part != nullptr) {
-                    store_columns(a.part + (partRow + n) * a.dim, d, a.dim, fours, v);
+                    store_columns(a.part + (partRow + n) * a.partDim, d, a.partDim, true, v);
                 } else if constexpr (P == 1) {
                     store_columns(static_cast<BF16*>(a.out) + (int64_t)n * a.dim, d, a.dim, fours, v);
                 } else {
@@ -669,46 +670,45 @@ __global__ __launch_bounds__(kLossThreads, OCC) void k_softmax_tiles(LossArgs a)
     }
 }
 
-// Joins the parts of the running sums and takes the target's score off: one wave per row of x.
-template <typename T>
+// Joins the parts of the running sums and takes the target's score off.  TEAM threads per row of x: a wave, or the block
+// where there are few rows, each with many parts.
+template <typename T, int TEAM>
 __global__ __launch_bounds__(kBlock) void k_softmax_loss_join(const float2* __restrict__ norm, int parts, int rows, int items,
                                                               int dim, const T* __restrict__ x, int64_t xStride,
                                                               const T* __restrict__ table, int64_t tableStride,
                                                               const int64_t* __restrict__ target, const float* __restrict__ bias,
                                                               float scale, float* __restrict__ loss, float* __restrict__ lse)
 {
-    const int n = blockIdx.x * (kBlock / kWave) + threadIdx.x / kWave;
-    const int lane = lane_id();
+    constexpr int kWaves = TEAM / kWave;
+    __shared__ float joined[kWaves][2];
+    const int n = blockIdx.x * (kBlock / TEAM) + threadIdx.x / TEAM;
+    const int lane = threadIdx.x % TEAM;
     if (n >= rows) {
         return;
     }
     const int64_t t = target[n];
-    if (t < 0 || t >= items) {   // no target: no loss, no gradient
+    const bool inside = t >= 0 && t < items;
+    const float b = inside && bias != nullptr ? bias[t] : 0.0f;
+    if (!inside || b <= kMaskedBelow) {
+        // no target: no loss; a target that is taken out: infinite; neither gives a gradient
         if (lane == 0) {
-            loss[n] = 0.0f;
+            loss[n] = inside ? INFINITY : 0.0f;
             lse[n] = INFINITY;
         }
-        return;
+        return;   // the whole team
     }
-    const float b = bias != nullptr ? bias[t] : 0.0f;
-    if (b <= kMaskedBelow) {   // the target cannot be had: infinite loss, no gradient
-        if (lane == 0) {
-            loss[n] = INFINITY;
-            lse[n] = INFINITY;
-        }
-        return;
+    float dot = 0.0f;
+    for (int d = lane; d < dim && lane < kWave; d += kWave) {
+        dot = __builtin_fmaf((float)x[n * xStride + d], (float)table[t * tableStride + d], dot);
     }
     float top = kFloor;
     float sum = 0.0f;
-    for (int p = lane; p < parts; p += kWave) {
+#pragma unroll 4
+    for (int p = lane; p < parts; p += TEAM) {
         const float2 v = norm[(int64_t)p * rows + n];
         const float now = fmaxf(top, v.x);
         sum = sum * exp2_fast(top - now) + v.y * exp2_fast(v.x - now);
         top = now;
-    }
-    float dot = 0.0f;
-    for (int d = lane; d < dim; d += kWave) {
-        dot = __builtin_fmaf((float)x[n * xStride + d], (float)table[t * tableStride + d], dot);
     }
 #pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) {
@@ -719,6 +719,19 @@ __global__ __launch_bounds__(kBlock) void k_softmax_loss_join(const float2* __re
         top = now;
         dot += __shfl_xor(dot, d, kWave);
     }
+    if constexpr (kWaves > 1) {
+        if (lane % kWave == 0) {
+            joined[lane / kWave][0] = top;
+            joined[lane / kWave][1] = sum;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) {
+            const float now = fmaxf(top, joined[w][0]);
+            sum = sum * exp2_fast(top - now) + joined[w][1] * exp2_fast(joined[w][0] - now);
+            top = now;
+        }
+    }
     if (lane == 0) {
         const float l = __builtin_fmaf(top, kLn2, logf(sum));
         loss[n] = l - __builtin_fmaf(dot, scale, b);
@@ -726,26 +739,24 @@ __global__ __launch_bounds__(kBlock) void k_softmax_loss_join(const float2* __re
     }
 }
 
-// out = factor(row) * sum of the parts, in the operands' type.  Four neighbouring values per thread (E = 4 where rows are
-// whole fours); the WAYS thread groups of a block take every WAYS-th part each and are joined in their order, so that few
-// values with many parts (few rows against a long table) still have many loads in flight.
-template <typename T, int E, int WAYS>
+// out = factor(row) * sum of the parts, in the operands' type.  Four columns per thread, 32 threads side by side; the WAYS
+// groups of 32 in a block take every WAYS-th part each and are joined in their order, so that few values with many parts
+// (few rows against a long table) still have many loads in flight.
+template <typename T, int WAYS>
 __global__ __launch_bounds__(kBlock) void k_softmax_grad_join(const float* __restrict__ part, int parts, int64_t count, int dim,
-                                                              const float* __restrict__ lse, const float* __restrict__ grad,
-                                                              float scale, T* __restrict__ out)
+                                                              int partDim, const float* __restrict__ lse,
+                                                              const float* __restrict__ grad, float scale, T* __restrict__ out)
 {
     constexpr int kWide = kBlock / WAYS;
-    typedef float FloatE __attribute__((ext_vector_type(E)));
-    typedef T OutE __attribute__((ext_vector_type(E)));
-    __shared__ FloatE sums[WAYS > 1 ? WAYS : 1][WAYS > 1 ? kWide : 1];
+    __shared__ Float4 sums[WAYS > 1 ? WAYS : 1][WAYS > 1 ? kWide : 1];
     const int way = threadIdx.x / kWide;
     const int at = threadIdx.x % kWide;
-    const int64_t i = ((int64_t)blockIdx.x * kWide + at) * E;
-    FloatE s = 0.0f;
+    const int64_t i = ((int64_t)blockIdx.x * kWide + at) * 4;
+    Float4 s = 0.0f;
     if (i < count) {
 #pragma unroll 8
         for (int p = way; p < parts; p += WAYS) {
-            s += *reinterpret_cast<const FloatE*>(part + p * count + i);
+            s += *reinterpret_cast<const Float4*>(part + p * count + i);
         }
     }
     if constexpr (WAYS > 1) {
@@ -762,31 +773,36 @@ __global__ __launch_bounds__(kBlock) void k_softmax_grad_join(const float* __res
     if (i >= count) {
         return;
     }
+    const int64_t n = i / partDim;
     float factor = 1.0f;
-    bool live = true;
     if (grad != nullptr) {
-        const int64_t n = i / dim;
-        live = lse[n] != INFINITY;
         factor = grad[n] * scale;
+        if (lse[n] == INFINITY) {   // takes no gradient, whatever grad holds
+            s = 0.0f;
+            factor = 0.0f;
+        }
     }
-    OutE o;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        o[e] = from_float<T>(live ? s[e] * factor : 0.0f);
-    }
-    *reinterpret_cast<OutE*>(out + i) = o;
+    store_columns(out + n * dim, (int)(i - n * partDim), dim, dim % 4 == 0, s * factor);
 }
 
-// Rows of `dim` elements at any stride -> rows of `padded` elements, the rest zero.
+// Rows of `dim` elements at any stride -> rows of `padded` elements (whole 16-byte pieces), the rest zero.  32 threads take
+// a row's pieces.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void k_pad_rows(const T* __restrict__ src, int64_t stride, int64_t rows, int dim, int padded,
                                                      T* __restrict__ dst)
 {
-    const int64_t i = (int64_t)blockIdx.x * kBlock + threadIdx.x;
-    const int64_t r = i / padded;
-    const int c = (int)(i - r * padded);
-    if (r < rows) {
-        dst[i] = c < dim ? src[r * stride + c] : from_float<T>(0.0f);
+    constexpr int kPer = 16 / sizeof(T);
+    const int64_t r = (int64_t)blockIdx.x * (kBlock / 32) + threadIdx.x / 32;
+    if (r >= rows) {
+        return;
+    }
+    for (int c = threadIdx.x % 32 * kPer; c < padded; c += 32 * kPer) {
+        Pack<T, kPer> v;
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) {
+            v.v[e] = c + e < dim ? src[r * stride + c + e] : from_float<T>(0.0f);
+        }
+        *reinterpret_cast<Pack<T, kPer>*>(dst + r * padded + c) = v;
     }
 }
 
@@ -882,8 +898,9 @@ static LossPlan plan_loss(int64_t rows, int64_t items, int32_t dim, int32_t dtyp
     p.atTable = round256(p.atX + (p.padX ? rows * p.padded * p.bytes : 0));
     p.atParts = round256(p.atTable + (p.padTable ? items * p.padded * p.bytes : 0));
     const int64_t norm = (int64_t)p.forward.parts * rows * (int64_t)sizeof(float2);
-    const int64_t dx = (int64_t)p.dx.parts * rows * dim * (int64_t)sizeof(float);
-    const int64_t dt = p.dt.parts > 1 ? (int64_t)p.dt.parts * items * dim * (int64_t)sizeof(float) : 0;
+    const int64_t pitch = cdiv(dim, 4) * 4 * (int64_t)sizeof(float);
+    const int64_t dx = (int64_t)p.dx.parts * rows * pitch;
+    const int64_t dt = p.dt.parts > 1 ? (int64_t)p.dt.parts * items * pitch : 0;
     p.forwardBytes = round256(p.atParts + norm);
     p.backwardBytes = round256(p.atParts + (dx > dt ? dx : dt));   // the two passes run one after the other
     return p;
@@ -979,8 +996,7 @@ static int check_loss(const char* name, int64_t rows, int64_t items, int32_t dim
 template <typename T>
 static int pad_operand(const void*& p, int64_t& stride, int64_t rows, int dim, int padded, void* to, hipStream_t stream)
 {
-    const int64_t grid = cdiv(rows * padded, kBlock);
-    RECSDK_REQUIRE(grid < (int64_t(1) << 31), RECSDK_EINVAL, "softmax loss: table too large for rows that need padding");
+    const int64_t grid = cdiv(rows, kBlock / 32);
     RECSDK_LAUNCH_AS("k_pad_rows", (k_pad_rows<T>), dim3((unsigned)grid), dim3(kBlock), stream, static_cast<const T*>(p), stride,
                      rows, dim, padded, static_cast<T*>(to));
     p = to;
@@ -988,30 +1004,25 @@ static int pad_operand(const void*& p, int64_t& stride, int64_t rows, int dim, i
     return RECSDK_OK;
 }
 
-template <typename T, int E, int WAYS>
-static int launch_grad_join(const float* part, int parts, int64_t count, int dim, const float* lse, const float* grad,
-                            float scale, T* out, hipStream_t stream)
+template <typename T, int WAYS>
+static int launch_grad_join(const float* part, int parts, int64_t rows, int dim, const float* lse, const float* grad,
+                            float scale, void* out, hipStream_t stream)
 {
-    const int64_t grid = cdiv(count, (int64_t)kBlock / WAYS * E);
+    const int partDim = (int)cdiv(dim, 4) * 4;
+    const int64_t grid = cdiv(rows * partDim, (int64_t)kBlock / WAYS * 4);
     RECSDK_REQUIRE(grid < (int64_t(1) << 31), RECSDK_EINVAL, "softmax loss: table too large for one launch");
-    RECSDK_LAUNCH_AS("k_softmax_grad_join", (k_softmax_grad_join<T, E, WAYS>), dim3((unsigned)grid), dim3(kBlock), stream, part,
-                     parts, count, dim, lse, grad, scale, out);
+    RECSDK_LAUNCH_AS("k_softmax_grad_join", (k_softmax_grad_join<T, WAYS>), dim3((unsigned)grid), dim3(kBlock), stream, part,
+                     parts, rows * partDim, dim, partDim, lse, grad, scale, static_cast<T*>(out));
     return RECSDK_OK;
 }
 
 template <typename T>
-static int join_grad(const float* part, int parts, int64_t count, int dim, const float* lse, const float* grad, float scale,
+static int join_grad(const float* part, int parts, int64_t rows, int dim, const float* lse, const float* grad, float scale,
                      void* out, hipStream_t stream)
 {
-    T* o = static_cast<T*>(out);
-    const bool fours = dim % 4 == 0;
-    // 16 ways where there are parts for all of them
-    if (parts >= 16) {
-        return fours ? launch_grad_join<T, 4, 16>(part, parts, count, dim, lse, grad, scale, o, stream)
-                     : launch_grad_join<T, 1, 16>(part, parts, count, dim, lse, grad, scale, o, stream);
-    }
-    return fours ? launch_grad_join<T, 4, 1>(part, parts, count, dim, lse, grad, scale, o, stream)
-                 : launch_grad_join<T, 1, 1>(part, parts, count, dim, lse, grad, scale, o, stream);
+    // eight ways where there are parts for all of them
+    return parts >= 8 ? launch_grad_join<T, 8>(part, parts, rows, dim, lse, grad, scale, out, stream)
+                      : launch_grad_join<T, 1>(part, parts, rows, dim, lse, grad, scale, out, stream);
 }
 
 struct LossOperands {
@@ -1062,9 +1073,17 @@ static int run_forward(const LossPlan& plan, LossOperands o, int64_t rows, int64
     if (rc != RECSDK_OK) {
         return rc;
     }
-    RECSDK_LAUNCH_AS("k_softmax_loss_join", (k_softmax_loss_join<T>), dim3((unsigned)cdiv(rows, kBlock / kWave)), dim3(kBlock),
-                     stream, a.norm, plan.forward.parts, (int)rows, (int)items, dim, static_cast<const T*>(given.x),
-                     given.xStride, static_cast<const T*>(given.table), given.tableStride, target, bias, scale, loss, lse);
+    const T* x = static_cast<const T*>(given.x);
+    const T* table = static_cast<const T*>(given.table);
+    if (plan.forward.parts >= 4 * kWave) {
+        RECSDK_LAUNCH_AS("k_softmax_loss_join", (k_softmax_loss_join<T, kBlock>), dim3((unsigned)rows), dim3(kBlock), stream,
+                         a.norm, plan.forward.parts, (int)rows, (int)items, dim, x, given.xStride, table, given.tableStride,
+                         target, bias, scale, loss, lse);
+    } else {
+        RECSDK_LAUNCH_AS("k_softmax_loss_join", (k_softmax_loss_join<T, kWave>), dim3((unsigned)cdiv(rows, kBlock / kWave)),
+                         dim3(kBlock), stream, a.norm, plan.forward.parts, (int)rows, (int)items, dim, x, given.xStride, table,
+                         given.tableStride, target, bias, scale, loss, lse);
+    }
     return RECSDK_OK;
 }
 
@@ -1084,6 +1103,7 @@ static int run_backward(const LossPlan& plan, LossOperands o, int64_t rows, int6
     a.lse = lse;
     a.grad = grad;
     a.scale = scale;
+    a.partDim = (int)cdiv(dim, 4) * 4;
     float* part = reinterpret_cast<float*>(workspace + plan.atParts);
     if (dx != nullptr) {
         a.own = o.x;
@@ -1097,7 +1117,7 @@ static int run_backward(const LossPlan& plan, LossOperands o, int64_t rows, int6
         if (rc != RECSDK_OK) {
             return rc;
         }
-        rc = join_grad<T>(part, plan.dx.parts, rows * dim, dim, lse, grad, scale, dx, stream);
+        rc = join_grad<T>(part, plan.dx.parts, rows, dim, lse, grad, scale, dx, stream);
         if (rc != RECSDK_OK) {
             return rc;
         }
@@ -1116,7 +1136,7 @@ static int run_backward(const LossPlan& plan, LossOperands o, int64_t rows, int6
             return rc;
         }
         if (a.part != nullptr) {
-            return join_grad<T>(part, plan.dt.parts, items * dim, dim, nullptr, nullptr, scale, dtable, stream);
+            return join_grad<T>(part, plan.dt.parts, items, dim, nullptr, nullptr, scale, dtable, stream);
         }
     }
     return RECSDK_OK;
@@ -1190,8 +1210,8 @@ extern "C" int recsdk_softmax_loss_backward(const float* d_grad_loss, const void
         if (d_dtable != nullptr) {
             RECSDK_REQUIRE(aligned16(d_dtable), RECSDK_EINVAL, "recsdk_softmax_loss_backward: dtable must be 16-byte aligned");
             return dtype == RECSDK_DT_F32
-                       ? join_grad<float>(nullptr, 0, items * dim, dim, nullptr, nullptr, scale, d_dtable, s)
-                       : join_grad<BF16>(nullptr, 0, items * dim, dim, nullptr, nullptr, scale, d_dtable, s);
+                       ? join_grad<float>(nullptr, 0, items, dim, nullptr, nullptr, scale, d_dtable, s)
+                       : join_grad<BF16>(nullptr, 0, items, dim, nullptr, nullptr, scale, d_dtable, s);
         }
         return RECSDK_OK;
     }
