@@ -67,6 +67,50 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, E>& r)
     }
 }
 
+// v + the same of the lane D away (D a power of two; groups of 2 D lanes end up with one value when the smaller steps were
+// taken before).  Within 16 lanes by data-parallel moves, across them by the row swaps: no trip through LDS, whose latency
+// a short row's two reductions would wait for ten times.
+template <int D>
+__device__ __forceinline__ float add_across(float v)
+{
+    if constexpr (D < 16) {
+        // quad permutations 1 0 3 2 and 2 3 0 1, then mirrors of 8 and of 16 lanes
+        constexpr int kCtrl = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x140;
+        return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xf, 0xf, true));
+    } else if constexpr (D == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    } else {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+}
+
+// Sum over aligned groups of G <= 64 lanes, in every lane of them.
+template <int G>
+__device__ __forceinline__ float group_sum(float v)
+{
+    if constexpr (G > 1) {
+        v = add_across<1>(v);
+    }
+    if constexpr (G > 2) {
+        v = add_across<2>(v);
+    }
+    if constexpr (G > 4) {
+        v = add_across<4>(v);
+    }
+    if constexpr (G > 8) {
+        v = add_across<8>(v);
+    }
+    if constexpr (G > 16) {
+        v = add_across<16>(v);
+    }
+    if constexpr (G > 32) {
+        v = add_across<32>(v);
+    }
+    return v;
+}
+
 #endif  // __HIPCC__
 
 }  // namespace recsdk

@@ -5,12 +5,15 @@
 //   backward   g = dy weight;  dx = rstd (g - sum g / D - hat sum (g hat) / D);  dweight = sum_rows dy hat;  dbias = sum_rows dy
 //
 // Rows are held in registers between their one read and their one write: a team of G threads per row, every thread K
-// packs of E columns (16 bytes where the rows are aligned to that, single elements where they are not), the variance
-// from the differences and not from the squares.  A team walks rows at a fixed stride, keeps its columns of weight and
-// bias in registers and has the next row's loads in flight while it reduces the present one.  In the backward pass the
-// same threads sum their columns of dweight and dbias over the team's rows; the teams of a block are joined in LDS, the
-// blocks' sums go to the workspace and a second kernel adds them in the order of the blocks: no atomics, so a call
-// gives the same bits every time.  All sums are held in 32 bits; every result is rounded once.
+// packs of 16 bytes, the variance from the differences and not from the squares.  A team walks rows at a fixed stride,
+// keeps its columns of weight and bias in registers and has the next rows' loads in flight while it reduces the present
+// ones (R rows side by side where a row is one pack per thread).  In the backward pass the same threads sum their columns
+// of dweight and dbias over the team's rows; the teams of a block are joined in LDS, the blocks' sums go to the workspace
+// and a second kernel adds them in the order of the blocks: no atomics, so a call gives the same bits every time.  All
+// sums are held in 32 bits; every result is rounded once.
+// Rows that do not start on 16-byte borders (an odd width) would move element by element, with an eighth of the bytes per
+// instruction; contiguous ones are staged instead: a block copies a span of whole rows, 16 KB of them, through LDS along the
+// 16-byte borders and works on elements there (30011 x 1001 fp16 forward: 50 -> STAGED_US us).
 // What bounds it: the row traffic (read x, write y; read dy and x, write dx).
 #include <math.h>
 
@@ -18,8 +21,13 @@
 
 namespace recsdk {
 
-constexpr int kNormBlocks = 512;        // blocks of the backward pass at most: each leaves 2 D sums in the workspace
-constexpr int kNormForwardBlocks = 2048;
+constexpr int kNormBlocks = 1024;       // blocks of the backward pass at most: each leaves 2 D sums in the workspace
+constexpr int kNormRowBlocks = 512;     // of them, where a block holds few rows' worth of registers
+constexpr int kNormForwardBlocks = 1024;
+constexpr int kNormSpanBlocks = 2048;
+constexpr int kSpanBytes = 16384;       // rows that a block stages at once
+constexpr int kSpanLoads = kSpanBytes / 16 / kBlock;
+constexpr int kSpanRows = kBlock;       // at most: one thread fetches a row's statistics
 constexpr int kReduceCols = 64;         // columns per block of the joining kernel
 constexpr int kReduceWaves = 16;
 
@@ -39,30 +47,32 @@ struct NormRows {
     float* part;        // [blocks][2][dim]
 };
 
-// Sum over the G threads of a team.  G > 64: the team is the block, `smem` holds two floats per wave.
-template <int G>
-__device__ __forceinline__ void team_sum2(float& a, float& b, float* smem)
+// Sums over the G threads of a team.  G > 64: the team is the block, `smem` holds N floats per wave.
+template <int G, int N>
+__device__ __forceinline__ void team_sum(float (&v)[N], float* smem)
 {
 #pragma unroll
-    for (int d = (G < kWave ? G : kWave) / 2; d > 0; d >>= 1) {
-        a += __shfl_xor(a, d, kWave);
-        b += __shfl_xor(b, d, kWave);
+    for (int n = 0; n < N; ++n) {
+        v[n] = group_sum<(G < kWave ? G : kWave)>(v[n]);
     }
     if constexpr (G > kWave) {
         constexpr int kWaves = G / kWave;
         const int w = threadIdx.x / kWave;
         __syncthreads();   // the previous sums have been read
         if (lane_id() == 0) {
-            smem[2 * w] = a;
-            smem[2 * w + 1] = b;
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                smem[N * w + n] = v[n];
+            }
         }
         __syncthreads();
-        a = 0;
-        b = 0;
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) {
-            a += smem[2 * k];
-            b += smem[2 * k + 1];
+        for (int n = 0; n < N; ++n) {
+            v[n] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kWaves; ++k) {
+                v[n] += smem[N * k + n];
+            }
         }
     }
 }
@@ -73,90 +83,171 @@ __device__ __forceinline__ float param(const void* p, int64_t c, float none)
     return p != nullptr ? (float)static_cast<const W*>(p)[c] : none;
 }
 
-template <typename T, typename W, int E, int G, int K>
-__global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm(NormRows a)
+// A thread's values of weight or bias: pack k holds E of them (E = 1, or a whole aligned piece) from column first + k step on;
+// 0 past the row's end.  The loads are made at a clamped column, so that none of them waits behind a branch for another.
+template <typename W, int E, int K>
+__device__ __forceinline__ void params(const void* p, int first, int step, int dim, float none, float (&out)[K][E])
 {
-    constexpr int kTeams = G > kBlock ? 1 : kBlock / G;
-    __shared__ float smem[2 * (G > kWave ? G / kWave : 1)];
-    const int lane = threadIdx.x % G;
-    const int64_t teams = (int64_t)gridDim.x * kTeams;
-    int64_t row = (int64_t)blockIdx.x * kTeams + threadIdx.x / G;
-    if (G <= kWave && row >= a.rows) {
+    if (p == nullptr) {
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                out[k][e] = first + k * step < dim ? none : 0.0f;
+            }
+        }
         return;
     }
-    const int dim = a.dim;
-    float wt[K][E];
-    float bs[K][E];
+    const W* w = static_cast<const W*>(p);
+    constexpr int kPer = E * sizeof(W) >= 16 ? 16 / (int)sizeof(W) : E;
+    Pack<W, kPer> v[K][E / kPer];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int q = 0; q < E / kPer; ++q) {
+            v[k][q] = load_pack<W, kPer>(w + min(first + k * step, dim - E) + q * kPer);
+        }
+    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int c = (k * G + lane) * E + e;
-            wt[k][e] = c < dim ? param<W>(a.weight, c, 1.0f) : 0.0f;
-            bs[k][e] = c < dim ? param<W>(a.bias, c, 0.0f) : 0.0f;
+            out[k][e] = first + k * step < dim ? (float)v[k][e / kPer].v[e % kPer] : 0.0f;
         }
+    }
+}
+
+// The block's column sums: its teams' joined in LDS (`joined`: kTeams * G * K * E floats; one team: unused), then written.
+template <int E, int G, int K, int TEAMS>
+__device__ __forceinline__ void leave_parts(const NormRows& a, float* joined, const float (&dw)[K][E], const float (&db)[K][E])
+{
+    constexpr int kCols = G * K * E;
+    const int team = threadIdx.x / G;
+    float* part = a.part + (int64_t)blockIdx.x * 2 * a.dim;
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+        if constexpr (TEAMS > 1) {
+            __syncthreads();
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int c = (k * G + (int)threadIdx.x % G) * E + e;
+                if (c < a.dim) {
+                    (TEAMS > 1 ? joined[team * kCols + c] : part[which * a.dim + c]) = which == 0 ? dw[k][e] : db[k][e];
+                }
+            }
+        }
+        if constexpr (TEAMS > 1) {
+            __syncthreads();
+            for (int c = threadIdx.x; c < a.dim; c += TEAMS * G) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int t = 0; t < TEAMS; ++t) {
+                    sum += joined[t * kCols + c];
+                }
+                part[which * a.dim + c] = sum;
+            }
+        }
+    }
+}
+
+// Rows that a team has in work at once.
+template <int G, int K, bool BACK>
+constexpr int kNormRows = G > kWave ? 1 : K == 1 ? (BACK ? 2 : 4) : K == 2 && !BACK ? 2 : 1;
+
+template <typename T, typename W, int E, int G, int K>
+__global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm(NormRows a)
+{
+    constexpr int R = kNormRows<G, K, false>;
+    constexpr int kTeams = G > kBlock ? 1 : kBlock / G;
+    __shared__ float smem[G > kWave ? R * G / kWave : 1];
+    const int64_t teams = (int64_t)gridDim.x * kTeams;
+    int64_t row = (int64_t)blockIdx.x * kTeams + threadIdx.x / G;
+    if (row >= a.rows) {
+        return;   // the whole team
     }
     const T* x = static_cast<const T*>(a.x);
     T* y = static_cast<T*>(a.y);
+    const int dim = a.dim;
+    const int first = threadIdx.x % G * E;   // pack k starts at column first + k G E
+    float wt[K][E];
+    float bs[K][E];
+    params<W, E, K>(a.weight, first, G * E, dim, 1.0f, wt);
+    params<W, E, K>(a.bias, first, G * E, dim, 0.0f, bs);
     const float inv = 1.0f / (float)dim;
-    Pack<T, E> next[K];
+    Pack<T, E> next[R][K];
     auto fetch = [&](int64_t r) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * G + lane) * E;
-            if (c < dim) {
-                next[k] = load_pack<T, E>(x + r * a.stride + c);
+        for (int i = 0; i < R; ++i) {
+            const int64_t at = r + i * teams;
+            if (at < a.rows) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const int c = first + k * G * E;
+                    if (c < dim) {
+                        next[i][k] = load_pack<T, E>(x + at * a.stride + c);
+                    }
+                }
             }
         }
     };
-    if (row < a.rows) {
-        fetch(row);
-    }
-    for (; row < a.rows; row += teams) {
-        float v[K][E];
-        float sum = 0.0f;
-        float none = 0.0f;
+    fetch(row);
+    for (; row < a.rows; row += R * teams) {
+        float v[R][K][E];
+        float mean[R];
+        float rstd[R];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const bool in = (k * G + lane) * E < dim;
+        for (int i = 0; i < R; ++i) {
+            mean[i] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                v[k][e] = in ? (float)next[k].v[e] : 0.0f;
-                sum += v[k][e];
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    v[i][k][e] = first + k * G * E < dim ? (float)next[i][k].v[e] : 0.0f;
+                    mean[i] += v[i][k][e];
+                }
             }
         }
-        if (row + teams < a.rows) {
-            fetch(row + teams);
-        }
-        team_sum2<G>(sum, none, smem);
-        const float mean = sum * inv;
-        float sq = 0.0f;
+        fetch(row + R * teams);
+        team_sum<G>(mean, smem);
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const bool in = (k * G + lane) * E < dim;
+        for (int i = 0; i < R; ++i) {
+            mean[i] *= inv;
+            rstd[i] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                v[k][e] = in ? v[k][e] - mean : 0.0f;
-                sq = __builtin_fmaf(v[k][e], v[k][e], sq);
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    v[i][k][e] = first + k * G * E < dim ? v[i][k][e] - mean[i] : 0.0f;
+                    rstd[i] = __builtin_fmaf(v[i][k][e], v[i][k][e], rstd[i]);
+                }
             }
         }
-        team_sum2<G>(sq, none, smem);
-        const float rstd = 1.0f / sqrtf(sq * inv + a.eps);
+        team_sum<G>(rstd, smem);
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * G + lane) * E;
-            if (c < dim) {
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = row + i * teams;
+            if (r >= a.rows) {
+                break;
+            }
+            rstd[i] = 1.0f / sqrtf(rstd[i] * inv + a.eps);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
                 Pack<T, E> out;
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
-                    out.v[e] = from_float<T>(__builtin_fmaf(v[k][e] * rstd, wt[k][e], bs[k][e]));
+                    out.v[e] = from_float<T>(__builtin_fmaf(v[i][k][e] * rstd[i], wt[k][e], bs[k][e]));
                 }
-                store_pack<T, E>(y + row * dim + c, out);
+                if (first + k * G * E < dim) {
+                    store_pack<T, E>(y + r * dim + first + k * G * E, out);
+                }
             }
-        }
-        if (lane == 0 && a.mean != nullptr) {
-            a.mean[row] = mean;
-            a.rstd[row] = rstd;
+            if (threadIdx.x % G == 0 && a.mean != nullptr) {
+                a.mean[r] = mean[i];
+                a.rstd[r] = rstd[i];
+            }
         }
     }
 }
@@ -164,13 +255,14 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm(NormRows
 template <typename T, typename W, int E, int G, int K>
 __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm_backward(NormRows a)
 {
+    constexpr int R = kNormRows<G, K, true>;
     constexpr int kThreads = G > kBlock ? G : kBlock;
     constexpr int kTeams = kThreads / G;
     constexpr int kCols = G * K * E;   // columns a team covers
     // the teams' column sums, joined at the end (one team per block: nothing to join)
-    __shared__ float joined[kTeams > 1 ? (kTeams * kCols > 8192 ? 8192 : kTeams * kCols) : 1];
-    __shared__ float smem[2 * (G > kWave ? G / kWave : 1)];
-    const int lane = threadIdx.x % G;
+    __shared__ float joined[kTeams > 1 ? kTeams * kCols : 1];
+    static_assert(kTeams == 1 || kTeams * kCols <= 8192, "the teams' sums fit the LDS array");
+    __shared__ float smem[G > kWave ? 2 * R * G / kWave : 1];
     const int team = threadIdx.x / G;
     const int64_t teams = (int64_t)gridDim.x * kTeams;
     const int dim = a.dim;
@@ -178,117 +270,368 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm_backward
     const T* x = static_cast<const T*>(a.x);
     const T* dy = static_cast<const T*>(a.grad);
     T* dx = static_cast<T*>(a.dx);
+    int64_t row = (int64_t)blockIdx.x * kTeams + team;
+    const int first = threadIdx.x % G * E;   // pack k starts at column first + k G E
     float wt[K][E];
     float dw[K][E];
     float db[K][E];
+    params<W, E, K>(a.weight, first, G * E, dim, 1.0f, wt);
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int c = (k * G + lane) * E + e;
-            wt[k][e] = c < dim ? param<W>(a.weight, c, 1.0f) : 0.0f;
             dw[k][e] = 0.0f;
             db[k][e] = 0.0f;
         }
     }
-    Pack<T, E> nx[K];
-    Pack<T, E> ng[K];
-    float nmean = 0.0f;
-    float nrstd = 0.0f;
-    auto fetch = [&](int64_t r) {
+    Pack<T, E> nx[R][K];
+    Pack<T, E> ng[R][K];
+    float nmean[R];
+    float nrstd[R];
+    auto fetch = [&](int64_t from) {
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (k * G + lane) * E;
-            if (c < dim) {
-                nx[k] = load_pack<T, E>(x + r * a.stride + c);
-                ng[k] = load_pack<T, E>(dy + r * dim + c);
+        for (int i = 0; i < R; ++i) {
+            const int64_t r = from + i * teams;
+            if (r < a.rows) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const int c = first + k * G * E;
+                    if (c < dim) {
+                        nx[i][k] = load_pack<T, E>(x + r * a.stride + c);
+                        ng[i][k] = load_pack<T, E>(dy + r * dim + c);
+                    }
+                }
+                nmean[i] = a.mean[r];
+                nrstd[i] = a.rstd[r];
             }
         }
-        nmean = a.mean[r];
-        nrstd = a.rstd[r];
     };
-    int64_t row = (int64_t)blockIdx.x * kTeams + team;
-    if (row < a.rows) {
-        fetch(row);
-    }
-    for (; row < a.rows; row += teams) {
-        float hat[K][E];
-        float g[K][E];
-        const float rstd = nrstd;
-        float s0 = 0.0f;
-        float s1 = 0.0f;
+    fetch(row);
+    for (; row < a.rows; row += R * teams) {
+        float hat[R][K][E];
+        float g[R][K][E];
+        float s[2 * R];
+        float rstd[R];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const bool in = (k * G + lane) * E < dim;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                hat[k][e] = in ? ((float)nx[k].v[e] - nmean) * rstd : 0.0f;
-                const float d = in ? (float)ng[k].v[e] : 0.0f;
-                dw[k][e] = __builtin_fmaf(d, hat[k][e], dw[k][e]);
-                db[k][e] += d;
-                g[k][e] = d * wt[k][e];
-                s0 += g[k][e];
-                s1 = __builtin_fmaf(g[k][e], hat[k][e], s1);
-            }
-        }
-        if (row + teams < a.rows) {
-            fetch(row + teams);
-        }
-        if (dx != nullptr) {
-            team_sum2<G>(s0, s1, smem);
-            s0 *= inv;
-            s1 *= inv;
+        for (int i = 0; i < R; ++i) {
+            const bool here = row + i * teams < a.rows;
+            rstd[i] = nrstd[i];
+            s[2 * i] = 0.0f;
+            s[2 * i + 1] = 0.0f;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int c = (k * G + lane) * E;
-                if (c < dim) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) {
+                    const bool in = first + k * G * E < dim && (R == 1 || here);
+                    hat[i][k][e] = in ? ((float)nx[i][k].v[e] - nmean[i]) * rstd[i] : 0.0f;
+                    const float d = in ? (float)ng[i][k].v[e] : 0.0f;
+                    dw[k][e] = __builtin_fmaf(d, hat[i][k][e], dw[k][e]);
+                    db[k][e] += d;
+                    g[i][k][e] = d * wt[k][e];
+                    s[2 * i] += g[i][k][e];
+                    s[2 * i + 1] = __builtin_fmaf(g[i][k][e], hat[i][k][e], s[2 * i + 1]);
+                }
+            }
+        }
+        fetch(row + R * teams);
+        if (dx != nullptr) {
+            team_sum<G>(s, smem);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int64_t r = row + i * teams;
+                if (r >= a.rows) {
+                    break;
+                }
+                const float s0 = s[2 * i] * inv;
+                const float s1 = s[2 * i + 1] * inv;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
                     Pack<T, E> out;
 #pragma unroll
                     for (int e = 0; e < E; ++e) {
-                        out.v[e] = from_float<T>(rstd * (g[k][e] - s0 - hat[k][e] * s1));
+                        out.v[e] = from_float<T>(rstd[i] * (g[i][k][e] - s0 - hat[i][k][e] * s1));
                     }
-                    store_pack<T, E>(dx + row * dim + c, out);
+                    if (first + k * G * E < dim) {
+                        store_pack<T, E>(dx + r * dim + first + k * G * E, out);
+                    }
                 }
             }
         }
     }
-    if (a.part == nullptr) {
-        return;
+    if (a.part != nullptr) {
+        leave_parts<E, G, K, kTeams>(a, joined, dw, db);
     }
-    float* part = a.part + (int64_t)blockIdx.x * 2 * dim;
+}
+
+// ---- staged rows ------------------------------------------------------------------------------------------------------
+// A span of contiguous rows on its way between memory and LDS.  It starts `lead` elements behind a 16-byte border and moves
+// in pieces along those borders: reads take whole pieces also where a neighbouring span has part of one, writes do not;
+// what is left, pieces that reach past the buffer (reads) or the span (writes), is a few elements, one thread each.
+template <typename T>
+struct Span {
+    static constexpr int kPer = 16 / sizeof(T);
+    const T* origin;   // the border at or before the first element
+    int before;        // elements of the buffer, from origin on, as far as a span can reach: [before, behind)
+    int behind;
+    int lead;
+    int count;         // elements of the span
+    __device__ __forceinline__ Span(const T* buffer, int64_t total, int64_t from, int n)
+    {
+        lead = (int)(reinterpret_cast<uintptr_t>(buffer + from) % 16 / sizeof(T));
+        origin = buffer + from - lead;
+        before = from < lead ? lead - (int)from : 0;
+        behind = (int)min(total - from + lead, (int64_t)kSpanBytes);
+        count = n;
+    }
+    __device__ __forceinline__ int pieces() const { return (lead + count + kPer - 1) / kPer; }
+    __device__ __forceinline__ bool whole(int piece) const
+    {
+        return piece * kPer >= before && piece * kPer + kPer <= behind;
+    }
+    __device__ __forceinline__ void load(Word4 (&r)[kSpanLoads]) const
+    {
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-        if constexpr (kTeams == 1) {
+        for (int q = 0; q < kSpanLoads; ++q) {
+            const int i = q * kBlock + threadIdx.x;
+            if (i < pieces() && whole(i)) {
+                r[q] = *reinterpret_cast<const Word4*>(origin + i * kPer);
+            }
+        }
+    }
+    __device__ __forceinline__ void place(const Word4 (&r)[kSpanLoads], T* lds) const
+    {
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
+        for (int q = 0; q < kSpanLoads; ++q) {
+            const int i = q * kBlock + threadIdx.x;
+            if (i < pieces() && whole(i)) {
+                *reinterpret_cast<Word4*>(lds + i * kPer) = r[q];
+            }
+        }
+        edges([&](int piece) { return !whole(piece); }, [&](int e) { lds[e] = origin[e]; });
+    }
+    // from LDS (laid out like `place` leaves it) to the same place of another buffer
+    __device__ __forceinline__ void store(const T* lds, T* to) const
+    {
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const int c = (k * G + lane) * E + e;
-                    if (c < dim) {
-                        part[which * dim + c] = which == 0 ? dw[k][e] : db[k][e];
+        for (int q = 0; q < kSpanLoads; ++q) {
+            const int i = q * kBlock + threadIdx.x;
+            if (i < pieces() && i * kPer >= lead && i * kPer + kPer <= lead + count) {
+                __builtin_nontemporal_store(*reinterpret_cast<const Word4*>(lds + i * kPer),
+                                            reinterpret_cast<Word4*>(to - lead + i * kPer));
+            }
+        }
+        edges([&](int piece) { return piece * kPer < lead || piece * kPer + kPer > lead + count; },
+              [&](int e) { to[e - lead] = lds[e]; });
+    }
+    // The span's elements in its first and in its last piece, where those ask for it: one thread each.
+    template <typename Asks, typename Move>
+    __device__ __forceinline__ void edges(Asks asks, Move move) const
+    {
+        const int last = pieces() - 1;
+        const int piece = threadIdx.x < kPer ? 0 : last;
+        const int e = piece * kPer + (int)threadIdx.x % kPer;
+        if (threadIdx.x < 2 * kPer && (threadIdx.x < kPer || last > 0) && e >= lead && e < lead + count && asks(piece)) {
+            move(e);
+        }
+    }
+};
+
+// The span's rows lie in LDS; a team takes every kTeams-th of them, a thread columns lane, lane + G, ...
+template <typename T, typename W, int G, int K>
+__global__ __launch_bounds__(kBlock) void k_layer_norm_staged(NormRows a, int spanRows)
+{
+    constexpr int kTeams = kBlock / G;
+    constexpr int R = G > kWave || K > 8 ? 1 : 2;   // rows that a team has in work at once
+    __shared__ __attribute__((aligned(16))) T lds[kSpanBytes / sizeof(T)];
+    __shared__ float smem[G > kWave ? R * G / kWave : 1];
+    const int dim = a.dim;
+    const int lane = threadIdx.x % G;
+    const int64_t total = a.rows * dim;
+    float wt[K][1];
+    float bs[K][1];
+    params<W, 1, K>(a.weight, lane, G, dim, 1.0f, wt);
+    params<W, 1, K>(a.bias, lane, G, dim, 0.0f, bs);
+    const float inv = 1.0f / (float)dim;
+    Word4 raw[kSpanLoads];
+    const int64_t step = (int64_t)gridDim.x * spanRows;
+    int64_t row0 = (int64_t)blockIdx.x * spanRows;
+    auto span = [&](int64_t r0) {
+        return Span<T>(static_cast<const T*>(a.x), total, r0 * dim, (int)min((int64_t)spanRows, a.rows - r0) * dim);
+    };
+    if (row0 < a.rows) {
+        span(row0).load(raw);
+    }
+    for (; row0 < a.rows; row0 += step) {
+        const Span<T> here = span(row0);
+        const int rows = (int)min((int64_t)spanRows, a.rows - row0);
+        here.place(raw, lds);
+        __syncthreads();
+        if (row0 + step < a.rows) {
+            span(row0 + step).load(raw);
+        }
+        for (int r0 = threadIdx.x / G; r0 < rows; r0 += R * kTeams) {
+            float v[R][K];
+            float mean[R];
+            float rstd[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const T* at = lds + here.lead + min(r0 + i * kTeams, rows - 1) * dim;
+                mean[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const float e = (float)at[min(k * G + lane, dim - 1)];
+                    v[i][k] = k * G + lane < dim ? e : 0.0f;
+                    mean[i] += v[i][k];
+                }
+            }
+            team_sum<G>(mean, smem);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                mean[i] *= inv;
+                rstd[i] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    v[i][k] = k * G + lane < dim ? v[i][k] - mean[i] : 0.0f;
+                    rstd[i] = __builtin_fmaf(v[i][k], v[i][k], rstd[i]);
+                }
+            }
+            team_sum<G>(rstd, smem);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int r = r0 + i * kTeams;
+                if (r >= rows) {
+                    break;
+                }
+                T* at = lds + here.lead + r * dim;
+                rstd[i] = 1.0f / sqrtf(rstd[i] * inv + a.eps);
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    if (k * G + lane < dim) {
+                        at[k * G + lane] = from_float<T>(__builtin_fmaf(v[i][k] * rstd[i], wt[k][0], bs[k][0]));
+                    }
+                }
+                if (lane == 0 && a.mean != nullptr) {
+                    a.mean[row0 + r] = mean[i];
+                    a.rstd[row0 + r] = rstd[i];
+                }
+            }
+        }
+        __syncthreads();
+        here.store(lds, static_cast<T*>(a.y) + row0 * dim);
+        __syncthreads();
+    }
+}
+
+template <typename T, typename W, int G, int K>
+__global__ __launch_bounds__(kBlock) void k_layer_norm_backward_staged(NormRows a, int spanRows)
+{
+    constexpr int kTeams = kBlock / G;
+    constexpr int R = G > kWave || K > 8 ? 1 : 2;
+    __shared__ __attribute__((aligned(16))) T lds[2][kSpanBytes / sizeof(T)];
+    __shared__ float stats[2][kSpanRows];
+    __shared__ float smem[G > kWave ? 2 * R * G / kWave : 1];
+    static_assert(kTeams == 1 || kTeams * G * K * sizeof(float) <= 2 * kSpanBytes, "the teams' sums fit the span's LDS");
+    const int dim = a.dim;
+    const int lane = threadIdx.x % G;
+    const int64_t total = a.rows * dim;
+    float wt[K][1];
+    float dw[K][1];
+    float db[K][1];
+    params<W, 1, K>(a.weight, lane, G, dim, 1.0f, wt);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        dw[k][0] = 0.0f;
+        db[k][0] = 0.0f;
+    }
+    const float inv = 1.0f / (float)dim;
+    Word4 rawX[kSpanLoads];
+    Word4 rawG[kSpanLoads];
+    const int64_t step = (int64_t)gridDim.x * spanRows;
+    int64_t row0 = (int64_t)blockIdx.x * spanRows;
+    auto span = [&](const void* p, int64_t r0) {
+        return Span<T>(static_cast<const T*>(p), total, r0 * dim, (int)min((int64_t)spanRows, a.rows - r0) * dim);
+    };
+    float rawMean = 0.0f;
+    float rawRstd = 0.0f;
+    auto fetch = [&](int64_t r0) {
+        span(a.x, r0).load(rawX);
+        span(a.grad, r0).load(rawG);
+        const int64_t r = min(r0 + (int)threadIdx.x, a.rows - 1);
+        rawMean = a.mean[r];
+        rawRstd = a.rstd[r];
+    };
+    if (row0 < a.rows) {
+        fetch(row0);
+    }
+    for (; row0 < a.rows; row0 += step) {
+        const Span<T> sx = span(a.x, row0);
+        const Span<T> sg = span(a.grad, row0);
+        const int rows = (int)min((int64_t)spanRows, a.rows - row0);
+        sx.place(rawX, lds[0]);
+        sg.place(rawG, lds[1]);
+        stats[0][threadIdx.x] = rawMean;
+        stats[1][threadIdx.x] = rawRstd;
+        __syncthreads();
+        if (row0 + step < a.rows) {
+            fetch(row0 + step);
+        }
+        for (int r0 = threadIdx.x / G; r0 < rows; r0 += R * kTeams) {
+            float hat[R][K];
+            float g[R][K];
+            float s[2 * R];
+            float rstd[R];
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const bool here = r0 + i * kTeams < rows;
+                const int r = here ? r0 + i * kTeams : r0;
+                const T* x = lds[0] + sx.lead + r * dim;
+                const T* dy = lds[1] + sg.lead + r * dim;
+                const float mean = stats[0][r];
+                rstd[i] = stats[1][r];
+                s[2 * i] = 0.0f;
+                s[2 * i + 1] = 0.0f;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    const bool in = k * G + lane < dim && here;
+                    const int c = min(k * G + lane, dim - 1);
+                    const float ex = (float)x[c];
+                    const float eg = (float)dy[c];
+                    hat[i][k] = in ? (ex - mean) * rstd[i] : 0.0f;
+                    const float d = in ? eg : 0.0f;
+                    dw[k][0] = __builtin_fmaf(d, hat[i][k], dw[k][0]);
+                    db[k][0] += d;
+                    g[i][k] = d * wt[k][0];
+                    s[2 * i] += g[i][k];
+                    s[2 * i + 1] = __builtin_fmaf(g[i][k], hat[i][k], s[2 * i + 1]);
+                }
+            }
+            if (a.dx != nullptr) {
+                team_sum<G>(s, smem);
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    if (r0 + i * kTeams >= rows) {
+                        break;
+                    }
+                    T* dy = lds[1] + sg.lead + (r0 + i * kTeams) * dim;
+                    const float s0 = s[2 * i] * inv;
+                    const float s1 = s[2 * i + 1] * inv;
+#pragma unroll
+                    for (int k = 0; k < K; ++k) {
+                        if (k * G + lane < dim) {
+                            dy[k * G + lane] = from_float<T>(rstd[i] * (g[i][k] - s0 - hat[i][k] * s1));
+                        }
                     }
                 }
             }
-        } else {
-            static_assert(kTeams * kCols <= 8192, "the teams' sums fit the LDS array");
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < K; ++k) {
-#pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    joined[team * kCols + (k * G + lane) * E + e] = which == 0 ? dw[k][e] : db[k][e];
-                }
-            }
-            __syncthreads();
-            for (int c = threadIdx.x; c < dim; c += kThreads) {
-                float s = 0.0f;
-#pragma unroll
-                for (int t = 0; t < kTeams; ++t) {
-                    s += joined[t * kCols + c];
-                }
-                part[which * dim + c] = s;
-            }
         }
+        __syncthreads();
+        if (a.dx != nullptr) {
+            sg.store(lds[1], static_cast<T*>(a.dx) + row0 * dim);
+            __syncthreads();
+        }
+    }
+    if (a.part != nullptr) {
+        leave_parts<1, G, K, kTeams>(a, reinterpret_cast<float*>(&lds[0][0]), dw, db);
     }
 }
 
@@ -300,20 +643,19 @@ __global__ __launch_bounds__(1024) void k_layer_norm_wide(NormRows a)
     const T* x = static_cast<const T*>(a.x) + (int64_t)blockIdx.x * a.stride;
     T* y = static_cast<T*>(a.y) + (int64_t)blockIdx.x * a.dim;
     const float inv = 1.0f / (float)a.dim;
-    float sum = 0.0f;
-    float none = 0.0f;
+    float sum[1] = {0.0f};
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
-        sum += (float)x[c];
+        sum[0] += (float)x[c];
     }
-    team_sum2<1024>(sum, none, smem);
-    const float mean = sum * inv;
-    float sq = 0.0f;
+    team_sum<1024>(sum, smem);
+    const float mean = sum[0] * inv;
+    sum[0] = 0.0f;
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
         const float d = (float)x[c] - mean;
-        sq = __builtin_fmaf(d, d, sq);
+        sum[0] = __builtin_fmaf(d, d, sum[0]);
     }
-    team_sum2<1024>(sq, none, smem);
-    const float rstd = 1.0f / sqrtf(sq * inv + a.eps);
+    team_sum<1024>(sum, smem);
+    const float rstd = 1.0f / sqrtf(sum[0] * inv + a.eps);
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
         y[c] = from_float<T>(__builtin_fmaf(((float)x[c] - mean) * rstd, param<W>(a.weight, c, 1.0f),
                                             param<W>(a.bias, c, 0.0f)));
@@ -333,16 +675,15 @@ __global__ __launch_bounds__(1024) void k_layer_norm_wide_dx(NormRows a)
     T* dx = static_cast<T*>(a.dx) + (int64_t)blockIdx.x * a.dim;
     const float mean = a.mean[blockIdx.x];
     const float rstd = a.rstd[blockIdx.x];
-    float s0 = 0.0f;
-    float s1 = 0.0f;
+    float s[2] = {0.0f, 0.0f};
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
         const float g = (float)dy[c] * param<W>(a.weight, c, 1.0f);
-        s0 += g;
-        s1 = __builtin_fmaf(g, ((float)x[c] - mean) * rstd, s1);
+        s[0] += g;
+        s[1] = __builtin_fmaf(g, ((float)x[c] - mean) * rstd, s[1]);
     }
-    team_sum2<1024>(s0, s1, smem);
-    s0 /= (float)a.dim;
-    s1 /= (float)a.dim;
+    team_sum<1024>(s, smem);
+    const float s0 = s[0] / (float)a.dim;
+    const float s1 = s[1] / (float)a.dim;
     for (int c = threadIdx.x; c < a.dim; c += 1024) {
         const float g = (float)dy[c] * param<W>(a.weight, c, 1.0f);
         dx[c] = from_float<T>(rstd * (g - s0 - ((float)x[c] - mean) * rstd * s1));
@@ -400,53 +741,34 @@ __global__ __launch_bounds__(kWave* kReduceWaves) void k_layer_norm_join(const f
     }
 }
 
-// What a row takes: threads per team and packs per thread, for packs of E elements; 0 threads = too wide.
-struct NormShape {
-    int team;
-    int packs;
-};
+// How a row is cut.  kWhole: packs of 16 bytes, every row on their borders; kStaged: contiguous rows that are not (every buffer's
+// first row equally far behind a border); kSingle: element by element, for rows with gaps that are not; kWide: rows past what
+// those hold in registers or LDS.
+enum NormCut { kWhole, kStaged, kSingle, kWide };
 
-static NormShape norm_shape(int dim, int e)
-{
-    const int packs = (int)cdiv(dim, e);
-    const int most = e == 1 ? 16 : 4;   // packs per thread: 16 to 32 values
-    if (packs <= 8) {
-        return {8, 1};
-    }
-    if (packs <= 16) {
-        return {16, 1};
-    }
-    if (packs <= 32) {
-        return {32, 1};
-    }
-    for (int k = 1; k <= most; k *= 2) {
-        if (packs <= 64 * k) {
-            return {64, k};
-        }
-    }
-    if (packs <= 256 * most) {
-        return {256, most};
-    }
-    if (packs <= 1024 * most) {
-        return {1024, most};
-    }
-    return {0, 0};
-}
-
-// Elements per access: whole 16 bytes where every row of every buffer starts on such a border.
 template <typename T>
-static int norm_pack(const NormRows& a)
+static NormCut norm_cut(const NormRows& a)
 {
-    const int e = 16 / (int)sizeof(T);
-    const bool ok = a.dim % e == 0 && a.stride % e == 0 && aligned16(a.x) && aligned16(a.y) && aligned16(a.grad) &&
-                    aligned16(a.dx);
-    return ok ? e : 1;
+    constexpr int kPer = 16 / (int)sizeof(T);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(a.x) % 16;
+    bool alike = at % sizeof(T) == 0;
+    for (const void* p : {static_cast<const void*>(a.y), a.grad, static_cast<const void*>(a.dx)}) {
+        alike = alike && (p == nullptr || reinterpret_cast<uintptr_t>(p) % 16 == at);
+    }
+    if (alike && at == 0 && a.dim % kPer == 0 && a.stride % kPer == 0 && aligned16(a.weight) && aligned16(a.bias)) {
+        return a.dim <= 2048 * kPer ? kWhole : kWide;
+    }
+    // a span and the elements between it and the borders at its ends
+    if (alike && (a.stride == a.dim || a.rows == 1) && ((int64_t)a.dim + 2 * kPer) * (int)sizeof(T) <= kSpanBytes) {
+        return kStaged;
+    }
+    return a.dim <= 4096 ? kSingle : kWide;
 }
 
-static int norm_backward_blocks(int64_t rows, int teamsPerBlock)
+static int norm_backward_blocks(int64_t rows, int rowsPerBlock, int most)
 {
-    const int64_t want = cdiv(rows, teamsPerBlock);
-    return (int)(want < kNormBlocks ? want : kNormBlocks);
+    const int64_t want = cdiv(rows, rowsPerBlock);
+    return (int)(want < most ? want : most);
 }
 
 template <typename T, typename W, int E, int G, int K, bool BACK>
@@ -454,60 +776,103 @@ static int launch_norm(const NormRows& a, int* blocks, hipStream_t stream)
 {
     constexpr int kThreads = G > kBlock ? G : kBlock;
     constexpr int kTeams = kThreads / G;
+    *blocks = norm_backward_blocks(a.rows, kTeams, BACK ? kNormRowBlocks : kNormForwardBlocks);
     if constexpr (BACK) {
-        *blocks = norm_backward_blocks(a.rows, kTeams);
         RECSDK_LAUNCH_AS("k_layer_norm_backward", (k_layer_norm_backward<T, W, E, G, K>), dim3((unsigned)*blocks), dim3(kThreads),
                          stream, a);
     } else {
-        const int64_t want = cdiv(a.rows, kTeams);
-        *blocks = (int)(want < kNormForwardBlocks ? want : kNormForwardBlocks);
         RECSDK_LAUNCH_AS("k_layer_norm", (k_layer_norm<T, W, E, G, K>), dim3((unsigned)*blocks), dim3(kThreads), stream, a);
     }
     return RECSDK_OK;
 }
 
-template <typename T, typename W, int E, bool BACK>
-static int dispatch_norm(const NormRows& a, int* blocks, hipStream_t stream)
+// 16 to 32 values per thread at most: the backward pass keeps five values per column and has to stay within the registers
+// of a block of 512 threads.
+template <typename T, typename W, bool BACK>
+static int launch_whole(const NormRows& a, int* blocks, hipStream_t stream)
 {
-    const NormShape s = norm_shape(a.dim, E);
-    constexpr int kMost = E == 1 ? 16 : 4;
-    switch (s.team) {
-        case 8:
-            return launch_norm<T, W, E, 8, 1, BACK>(a, blocks, stream);
-        case 16:
-            return launch_norm<T, W, E, 16, 1, BACK>(a, blocks, stream);
-        case 32:
-            return launch_norm<T, W, E, 32, 1, BACK>(a, blocks, stream);
-        case 64:
-            if (s.packs == 1) {
-                return launch_norm<T, W, E, 64, 1, BACK>(a, blocks, stream);
-            }
-            if (s.packs == 2) {
-                return launch_norm<T, W, E, 64, 2, BACK>(a, blocks, stream);
-            }
-            if (s.packs == 4) {
-                return launch_norm<T, W, E, 64, 4, BACK>(a, blocks, stream);
-            }
-            if constexpr (E == 1) {
-                if (s.packs == 8) {
-                    return launch_norm<T, W, E, 64, 8, BACK>(a, blocks, stream);
-                }
-                return launch_norm<T, W, E, 64, 16, BACK>(a, blocks, stream);
-            }
-            break;
-        case 256:
-            return launch_norm<T, W, E, 256, kMost, BACK>(a, blocks, stream);
-        case 1024:
-            return launch_norm<T, W, E, 1024, kMost, BACK>(a, blocks, stream);
-        default:
-            break;
+    constexpr int E = 16 / (int)sizeof(T);
+    const int packs = a.dim / E;
+    if (packs <= 4) {
+        return launch_norm<T, W, E, 4, 1, BACK>(a, blocks, stream);
     }
+    if (packs <= 8) {
+        return launch_norm<T, W, E, 8, 1, BACK>(a, blocks, stream);
+    }
+    if (packs <= 16) {
+        return launch_norm<T, W, E, 16, 1, BACK>(a, blocks, stream);
+    }
+    if (packs <= 32) {
+        return launch_norm<T, W, E, 32, 1, BACK>(a, blocks, stream);
+    }
+    if (packs <= 64) {
+        return launch_norm<T, W, E, 64, 1, BACK>(a, blocks, stream);
+    }
+    if (packs <= 128) {
+        return launch_norm<T, W, E, 64, 2, BACK>(a, blocks, stream);
+    }
+    if (packs <= 256) {
+        return launch_norm<T, W, E, 64, 4, BACK>(a, blocks, stream);
+    }
+    if (packs <= 1024) {
+        return launch_norm<T, W, E, 256, 4, BACK>(a, blocks, stream);
+    }
+    return launch_norm<T, W, E, 512, 4, BACK>(a, blocks, stream);
+}
+
+template <typename T, typename W, int G, int K, bool BACK>
+static int launch_spans(const NormRows& a, int* blocks, hipStream_t stream)
+{
+    constexpr int kPer = 16 / (int)sizeof(T);
+    const int fit = (kSpanBytes / (int)sizeof(T) - 2 * kPer) / a.dim;
+    const int spanRows = fit < kSpanRows ? fit : kSpanRows;
+    *blocks = norm_backward_blocks(a.rows, spanRows, BACK ? kNormBlocks : kNormSpanBlocks);
+    if constexpr (BACK) {
+        RECSDK_LAUNCH_AS("k_layer_norm_backward", (k_layer_norm_backward_staged<T, W, G, K>), dim3((unsigned)*blocks), dim3(kBlock),
+                         stream, a, spanRows);
+    } else {
+        RECSDK_LAUNCH_AS("k_layer_norm", (k_layer_norm_staged<T, W, G, K>), dim3((unsigned)*blocks), dim3(kBlock), stream, a,
+                         spanRows);
+    }
+    return RECSDK_OK;
+}
+
+template <typename T, typename W, bool BACK>
+static int launch_staged(const NormRows& a, int* blocks, hipStream_t stream)
+{
+    if (a.dim <= 16) {
+        return launch_spans<T, W, 4, 4, BACK>(a, blocks, stream);
+    }
+    if (a.dim <= 64) {
+        return launch_spans<T, W, 16, 4, BACK>(a, blocks, stream);
+    }
+    if (a.dim <= 128) {
+        return launch_spans<T, W, 16, 8, BACK>(a, blocks, stream);
+    }
+    if (a.dim <= 256) {
+        return launch_spans<T, W, 32, 8, BACK>(a, blocks, stream);
+    }
+    if (a.dim <= 512) {
+        return launch_spans<T, W, 64, 8, BACK>(a, blocks, stream);
+    }
+    if (a.dim <= 1024) {
+        return launch_spans<T, W, 64, 16, BACK>(a, blocks, stream);
+    }
+    if (a.dim <= 4096) {
+        return launch_spans<T, W, 256, 16, BACK>(a, blocks, stream);
+    }
+    return launch_spans<T, W, 256, 32, BACK>(a, blocks, stream);
+}
+
+template <typename T, typename W, bool BACK>
+static int launch_wide(const NormRows& a, int* blocks, hipStream_t stream)
+{
     if constexpr (BACK) {
         if (a.dx != nullptr) {
             RECSDK_LAUNCH_AS("k_layer_norm_wide_dx", (k_layer_norm_wide_dx<T, W>), dim3((unsigned)a.rows), dim3(1024), stream, a);
         }
         if (a.part != nullptr) {
-            *blocks = norm_backward_blocks(a.rows, 16);
+            *blocks = norm_backward_blocks(a.rows, 16, kNormBlocks);
             RECSDK_LAUNCH_AS("k_layer_norm_wide_params", (k_layer_norm_wide_params<T>),
                              dim3((unsigned)cdiv(a.dim, kBlock), (unsigned)*blocks), dim3(kBlock), stream, a);
         }
@@ -518,12 +883,28 @@ static int dispatch_norm(const NormRows& a, int* blocks, hipStream_t stream)
 }
 
 template <typename T, typename W, bool BACK>
+static int launch_rows(const NormRows& a, int* blocks, hipStream_t stream)
+{
+    switch (norm_cut<T>(a)) {
+        case kWhole:
+            return launch_whole<T, W, BACK>(a, blocks, stream);
+        case kStaged:
+            return launch_staged<T, W, BACK>(a, blocks, stream);
+        case kSingle:
+            return a.dim <= 256    ? launch_norm<T, W, 1, 64, 4, BACK>(a, blocks, stream)
+                   : a.dim <= 1024 ? launch_norm<T, W, 1, 64, 16, BACK>(a, blocks, stream)
+                                   : launch_norm<T, W, 1, 256, 16, BACK>(a, blocks, stream);
+        default:
+            return launch_wide<T, W, BACK>(a, blocks, stream);
+    }
+}
+
+template <typename T, typename W, bool BACK>
 static int run_norm_typed(const NormRows& a, void* dweight, void* dbias, hipStream_t stream)
 {
     int blocks = 0;
     if (a.rows > 0) {
-        const int rc = norm_pack<T>(a) == 1 ? dispatch_norm<T, W, 1, BACK>(a, &blocks, stream)
-                                            : dispatch_norm<T, W, 16 / (int)sizeof(T), BACK>(a, &blocks, stream);
+        const int rc = launch_rows<T, W, BACK>(a, &blocks, stream);
         if (rc != RECSDK_OK) {
             return rc;
         }
@@ -608,7 +989,7 @@ extern "C" int recsdk_layer_norm_workspace(int64_t rows, int32_t dim, int64_t* h
     using namespace recsdk;
     RECSDK_REQUIRE(h_bytes != nullptr, RECSDK_ENULL, "recsdk_layer_norm_workspace: NULL argument");
     RECSDK_REQUIRE(rows >= 0 && dim >= 1, RECSDK_EINVAL, "recsdk_layer_norm_workspace: bad sizes");
-    *h_bytes = (int64_t)norm_backward_blocks(rows, 1) * 2 * dim * (int64_t)sizeof(float);
+    *h_bytes = (int64_t)norm_backward_blocks(rows, 1, kNormBlocks) * 2 * dim * (int64_t)sizeof(float);
     return RECSDK_OK;
 }
 
