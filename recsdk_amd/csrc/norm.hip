@@ -13,7 +13,7 @@
 // sums are held in 32 bits; every result is rounded once.
 // Rows that do not start on 16-byte borders (an odd width) would move element by element, with an eighth of the bytes per
 // instruction; contiguous ones are staged instead: a block copies a span of whole rows, 16 KB of them, through LDS along the
-// 16-byte borders and works on elements there (30011 x 1001 fp16 forward: 50 -> STAGED_US us).
+// 16-byte borders and works on elements there (30011 x 1001 fp16 forward: 50 -> 31 us).
 // What bounds it: the row traffic (read x, write y; read dy and x, write dx).
 #include <math.h>
 
@@ -23,7 +23,7 @@ namespace recsdk {
 
 constexpr int kNormBlocks = 1024;       // blocks of the backward pass at most: each leaves 2 D sums in the workspace
 constexpr int kNormRowBlocks = 512;     // of them, where a block holds few rows' worth of registers
-constexpr int kNormForwardBlocks = 1024;
+constexpr int kNormForwardBlocks = 2048;
 constexpr int kNormSpanBlocks = 2048;
 constexpr int kSpanBytes = 16384;       // rows that a block stages at once
 constexpr int kSpanLoads = kSpanBytes / 16 / kBlock;
@@ -163,8 +163,8 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm(NormRows
     constexpr int R = kNormRows<G, K, false>;
     constexpr int kTeams = G > kBlock ? 1 : kBlock / G;
     __shared__ float smem[G > kWave ? R * G / kWave : 1];
-    const int64_t teams = (int64_t)gridDim.x * kTeams;
-    int64_t row = (int64_t)blockIdx.x * kTeams + threadIdx.x / G;
+    const int64_t step = (int64_t)gridDim.x * (R * kTeams);
+    int64_t row = (int64_t)blockIdx.x * (R * kTeams) + threadIdx.x / G;
     if (row >= a.rows) {
         return;   // the whole team
     }
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm(NormRows
     auto fetch = [&](int64_t r) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int64_t at = r + i * teams;
+            const int64_t at = r + i * kTeams;
             if (at < a.rows) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm(NormRows
         }
     };
     fetch(row);
-    for (; row < a.rows; row += R * teams) {
+    for (; row < a.rows; row += step) {
         float v[R][K][E];
         float mean[R];
         float rstd[R];
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm(NormRows
                 }
             }
         }
-        fetch(row + R * teams);
+        fetch(row + step);
         team_sum<G>(mean, smem);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm(NormRows
         team_sum<G>(rstd, smem);
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int64_t r = row + i * teams;
+            const int64_t r = row + i * kTeams;
             if (r >= a.rows) {
                 break;
             }
@@ -264,13 +264,13 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm_backward
     static_assert(kTeams == 1 || kTeams * kCols <= 8192, "the teams' sums fit the LDS array");
     __shared__ float smem[G > kWave ? 2 * R * G / kWave : 1];
     const int team = threadIdx.x / G;
-    const int64_t teams = (int64_t)gridDim.x * kTeams;
+    const int64_t step = (int64_t)gridDim.x * (R * kTeams);
     const int dim = a.dim;
     const float inv = 1.0f / (float)dim;
     const T* x = static_cast<const T*>(a.x);
     const T* dy = static_cast<const T*>(a.grad);
     T* dx = static_cast<T*>(a.dx);
-    int64_t row = (int64_t)blockIdx.x * kTeams + team;
+    int64_t row = (int64_t)blockIdx.x * (R * kTeams) + team;
     const int first = threadIdx.x % G * E;   // pack k starts at column first + k G E
     float wt[K][E];
     float dw[K][E];
@@ -291,7 +291,7 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm_backward
     auto fetch = [&](int64_t from) {
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const int64_t r = from + i * teams;
+            const int64_t r = from + i * kTeams;
             if (r < a.rows) {
 #pragma unroll
                 for (int k = 0; k < K; ++k) {
@@ -307,14 +307,14 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm_backward
         }
     };
     fetch(row);
-    for (; row < a.rows; row += R * teams) {
+    for (; row < a.rows; row += step) {
         float hat[R][K][E];
         float g[R][K][E];
         float s[2 * R];
         float rstd[R];
 #pragma unroll
         for (int i = 0; i < R; ++i) {
-            const bool here = row + i * teams < a.rows;
+            const bool here = row + i * kTeams < a.rows;
             rstd[i] = nrstd[i];
             s[2 * i] = 0.0f;
             s[2 * i + 1] = 0.0f;
@@ -333,12 +333,12 @@ __global__ __launch_bounds__(G > kBlock ? G : kBlock) void k_layer_norm_backward
                 }
             }
         }
-        fetch(row + R * teams);
+        fetch(row + step);
         if (dx != nullptr) {
             team_sum<G>(s, smem);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
-                const int64_t r = row + i * teams;
+                const int64_t r = row + i * kTeams;
                 if (r >= a.rows) {
                     break;
                 }
@@ -775,8 +775,8 @@ template <typename T, typename W, int E, int G, int K, bool BACK>
 static int launch_norm(const NormRows& a, int* blocks, hipStream_t stream)
 {
     constexpr int kThreads = G > kBlock ? G : kBlock;
-    constexpr int kTeams = kThreads / G;
-    *blocks = norm_backward_blocks(a.rows, kTeams, BACK ? kNormRowBlocks : kNormForwardBlocks);
+    constexpr int kRows = kThreads / G * kNormRows<G, K, BACK>;
+    *blocks = norm_backward_blocks(a.rows, kRows, BACK ? kNormRowBlocks : kNormForwardBlocks);
     if constexpr (BACK) {
         RECSDK_LAUNCH_AS("k_layer_norm_backward", (k_layer_norm_backward<T, W, E, G, K>), dim3((unsigned)*blocks), dim3(kThreads),
                          stream, a);
