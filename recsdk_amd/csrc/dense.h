@@ -67,6 +67,25 @@ __device__ __forceinline__ void store_pack(T* p, const Pack<T, E>& r)
     }
 }
 
+// Columns d .. d + 3 of a row, as far as it has them.
+template <typename T>
+__device__ __forceinline__ void store_columns(T* row, int d, int dim, bool fours, Float4 v)
+{
+    typedef T T4 __attribute__((ext_vector_type(4)));
+    if (fours) {
+        if (d < dim) {
+            *reinterpret_cast<T4*>(row + d) = T4{from_float<T>(v[0]), from_float<T>(v[1]), from_float<T>(v[2]), from_float<T>(v[3])};
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (d + j < dim) {
+                row[d + j] = from_float<T>(v[j]);
+            }
+        }
+    }
+}
+
 // v + the same of the lane D away (D a power of two; groups of 2 D lanes end up with one value when the smaller steps were
 // taken before).  Within 16 lanes by data-parallel moves, across them by the row swaps: no trip through LDS, whose latency
 // a short row's two reductions would wait for ten times.

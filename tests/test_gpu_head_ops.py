@@ -226,6 +226,46 @@ def check_loss(ops, x, table, target, bias, scale, grad):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [1, 16, 33, 64, 96, 100, 128, 160, 161, 192, 224, 225, 256])
+def test_softmax_loss_widths_of_few_rows(ops, kind, dim):
+    x, table, target, grad = loss_case(20, 333, dim, kind, dim)
+    check_loss(ops, x, table, target, None, 3 / math.sqrt(dim), grad)
+    bias = torch.randn(333, generator=torch.Generator().manual_seed(dim)).to(DEV)
+    check_loss(ops, x, table, target, bias, 3 / math.sqrt(dim), grad)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [72, 96, 129, 160, 192, 224])
+def test_softmax_loss_widths_with_a_bias(ops, kind, dim):
+    x, table, target, grad = loss_case(200, 333, dim, kind, dim)
+    bias = torch.randn(333, generator=torch.Generator().manual_seed(dim)).to(DEV)
+    bias[::7] = -math.inf
+    check_loss(ops, x, table, target, bias, 3 / math.sqrt(dim), grad)
+
+
+@pytest.mark.parametrize("big,small", [(1e15, 1e-15), (1e-18, 1e18), (1e-30, 1.0), (1e4, 1e4)])
+def test_softmax_loss_magnitudes_of_float32(ops, big, small):
+    x, table, target, grad = loss_case(100, 400, 64, "f32", 91)
+    scale = 0.4 / (big * small)
+    check_loss(ops, x * big, table * small, target, None, scale, grad)
+    # rows of very different sizes: the smallest take part with 2^-22 of themselves as long as they are 2^-18 of the largest
+    rise = torch.logspace(-4, 0, 400, device=DEV)[:, None]
+    check_loss(ops, x * big, table * small * rise, target, None, scale, grad)
+
+
+def test_softmax_loss_gradients_of_very_different_rows(ops):
+    """Gradients of loss from 1e-12 to 1e6, also negative ones and zeros: every item keeps the precision of its own rows."""
+    for kind in ("f32", "bf16"):
+        x, table, target, grad = loss_case(300, 350, 48, kind, 92)
+        grad = grad * torch.logspace(-12, 6, 300, device=DEV)
+        grad[::3] *= -1
+        grad[7::11] = 0
+        order = torch.randperm(300, generator=torch.Generator().manual_seed(1)).to(DEV)
+        for g in (grad, grad.flip(0).contiguous(), grad[order].contiguous()):
+            check_loss(ops, x, table, target, None, 0.5, g)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 @pytest.mark.parametrize("dim", [1, 7, 8, 16, 32, 36, 64, 68, 100, 128, 132, 200, 201, 255, 256])
 def test_softmax_loss_widths(ops, kind, dim):
     x, table, target, grad = loss_case(70, 333, dim, kind, dim)
