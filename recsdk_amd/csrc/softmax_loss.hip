@@ -5,6 +5,7 @@
 namespace recsdk {
 
 constexpr int kFewRows = 32;
+constexpr int kAbsMaxThreads = 1024;
 
 // Joins the parts of the running sums and takes the target's score off.  TEAM threads per row of x: a wave, or the block
 // where there are few rows, each with many parts.
@@ -144,31 +145,38 @@ __global__ __launch_bounds__(kBlock) void k_pad_rows(const T* __restrict__ src, 
 
 // Largest finite |value| of x (the first kAbsMaxParts blocks) and of the table, a part per block.  Rows that take no part are
 // left out: they may hold anything.  32 threads per row, 16 bytes each.
-__global__ __launch_bounds__(kBlock) void k_abs_max(const float* __restrict__ x, int64_t xStride, int rows,
+__global__ __launch_bounds__(kAbsMaxThreads) void k_abs_max(const float* __restrict__ x, int64_t xStride, int rows,
                                                     const float* __restrict__ table, int64_t tableStride, int items, int dim,
                                                     const int64_t* __restrict__ target, const float* __restrict__ bias,
                                                     float* __restrict__ parts)
 {
-    __shared__ float sums[kBlock / kWave];
-    constexpr int kStep = kAbsMaxParts * (kBlock / 32);
+    __shared__ float sums[kAbsMaxThreads / kWave];
+    constexpr int kStep = kAbsMaxParts * (kAbsMaxThreads / 32);
+    constexpr int kFlight = 4;   // rows whose loads are in flight at once
     const bool second = blockIdx.x >= kAbsMaxParts;
     const float* base = second ? table : x;
     const int64_t stride = second ? tableStride : xStride;
     const int count = second ? items : rows;
     float most = 0.0f;
-#pragma unroll 4
-    for (int r = blockIdx.x % kAbsMaxParts * (kBlock / 32) + threadIdx.x / 32; r < count; r += kStep) {
-        const bool live = second ? bias == nullptr || bias[r] > kMaskedBelow : (uint64_t)target[r] < (uint64_t)items;
-        float here = 0.0f;
+    for (int r0 = blockIdx.x % kAbsMaxParts * (kAbsMaxThreads / 32) + threadIdx.x / 32; r0 < count; r0 += kFlight * kStep) {
         for (int c = threadIdx.x % 32 * 4; c < dim; c += 128) {
-            const Float4 v = *reinterpret_cast<const Float4*>(base + r * stride + c);
+            Float4 v[kFlight];
+            bool live[kFlight];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float m = fabsf(v[j]);
-                here = m < INFINITY ? fmaxf(here, m) : here;   // not a NaN either
+            for (int q = 0; q < kFlight; ++q) {
+                const int64_t r = min((int64_t)r0 + (int64_t)q * kStep, (int64_t)count - 1);
+                v[q] = *reinterpret_cast<const Float4*>(base + r * stride + c);
+                live[q] = second ? bias == nullptr || bias[r] > kMaskedBelow : (uint64_t)target[r] < (uint64_t)items;
+            }
+#pragma unroll
+            for (int q = 0; q < kFlight; ++q) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float m = fabsf(v[q][j]);
+                    most = live[q] && m < INFINITY ? fmaxf(most, m) : most;   // not a NaN either
+                }
             }
         }
-        most = live ? fmaxf(most, here) : most;
     }
 #pragma unroll
     for (int d = kWave / 2; d > 0; d >>= 1) {
@@ -179,13 +187,18 @@ __global__ __launch_bounds__(kBlock) void k_abs_max(const float* __restrict__ x,
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        parts[blockIdx.x] = fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3]));
+#pragma unroll
+        for (int w = 1; w < kAbsMaxThreads / kWave; ++w) {
+            most = fmaxf(most, sums[w]);
+        }
+        parts[blockIdx.x] = most;
     }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 
 constexpr int kComputeUnits = 256;
+constexpr int kSplitTiles = 3;   // tiles of a split at least: what a block does before its first takes about as long
 
 static PassPlan plan_pass(int planes, int dim, int64_t owners, int64_t streams, int pass)
 {
@@ -204,7 +217,10 @@ static PassPlan plan_pass(int planes, int dim, int64_t owners, int64_t streams, 
     p.blocks = cdiv(owners, (int64_t)p.rowsPerWave * p.ownWaves);
     const int64_t tiles = cdiv(streams, tile_rows(planes, dp, p.ownWaves, pass));
     int64_t splits = (int64_t)kComputeUnits * resident_blocks(planes, dp, pass) / p.blocks;
-    splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
+    if (splits > tiles / kSplitTiles) {
+        splits = tiles / kSplitTiles;
+    }
+    splits = splits < 1 ? 1 : splits;
     p.tilesPerSplit = (int)cdiv(tiles, splits);
     p.splits = (int)cdiv(tiles, p.tilesPerSplit);
     p.parts = p.splits * (4 / p.ownWaves);
@@ -346,7 +362,7 @@ static int find_largest(const LossPlan& plan, const LossOperands& o, int64_t row
                         const float* bias, char* workspace, hipStream_t stream)
 {
     if (plan.planes == 2) {
-        RECSDK_LAUNCH_AS("k_abs_max", k_abs_max, dim3(2 * kAbsMaxParts), dim3(kBlock), stream, static_cast<const float*>(o.x),
+        RECSDK_LAUNCH_AS("k_abs_max", k_abs_max, dim3(2 * kAbsMaxParts), dim3(kAbsMaxThreads), stream, static_cast<const float*>(o.x),
                          o.xStride, (int)rows, static_cast<const float*>(o.table), o.tableStride, (int)items, dim, target, bias,
                          reinterpret_cast<float*>(workspace + plan.atMax));
     }

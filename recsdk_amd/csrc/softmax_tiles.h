@@ -324,63 +324,37 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
     const int tiles = (a.streams + TR - 1) / TR;
     const int t0 = split * a.tilesPerSplit;
     const int t1 = min(t0 + a.tilesPerSplit, tiles);   // t0 < t1: no split is empty
-    // the forward pass bounds scores by the largest product, so there a negative scale goes into the owner's rows
-    const bool turned = PASS == kLossForward && a.scale < 0.0f;
-    float c2 = (turned ? -a.scale : a.scale) * kLog2e;
-    float ownScale = 1.0f;
-    float streamScale = 1.0f;
-    if constexpr (P == 2) {
-        float* largest = &auxA[0][0];   // free until the first tile is placed
-        static_assert(kAbsMaxParts == kLossThreads, "one part per thread");
-        const float o = wave_max(a.ownMax[threadIdx.x]);
-        const float s = wave_max(a.streamMax[threadIdx.x]);
-        if (lane == 0) {
-            largest[wave] = o;
-            largest[4 + wave] = s;
-        }
-        __syncthreads();
-        ownScale = plane_scale(fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3])));
-        streamScale = plane_scale(fmaxf(fmaxf(largest[4], largest[5]), fmaxf(largest[6], largest[7])));
-        __syncthreads();
-        c2 = c2 / ownScale / streamScale;
-    }
     const bool biased = a.bias != nullptr;
     constexpr int kElement = P == 1 ? 2 : 4;
+    float ownMost = 0.0f;
+    float streamMost = 0.0f;
+    if constexpr (P == 2) {
+        static_assert(kAbsMaxParts == kLossThreads, "one part per thread");
+        ownMost = a.ownMax[threadIdx.x];
+        streamMost = a.streamMax[threadIdx.x];
+    }
 
-    // ---- the rows this wave owns ----
-    Frag<P> own[CB][KS][P];
-    int32_t ownTarget[CB];   // forward, dx
-    float ownShift[CB];      // dx: lse (base 2); dt: bias (base 2)
+    // ---- the rows this wave owns, as they come from memory: looked at once the first tile's loads are under way ----
+    int32_t ownTarget[CB];   // dx
+    float ownShift[CB];      // dx: lse; dt: bias
+    RowChunk<P> ownRaw[CB][KS];
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
-        const int n = ownBase + cb * 32 + col;
-        bool live = n < a.owners;
+        const int64_t n = min(ownBase + cb * 32 + col, a.owners - 1);
         ownTarget[cb] = -1;
         ownShift[cb] = 0.0f;
         if constexpr (PASS == kLossDx) {
-            ownShift[cb] = live ? a.lse[n] * kLog2e : INFINITY;
-            live = live && ownShift[cb] != INFINITY;
-            ownTarget[cb] = live ? (int32_t)a.target[n] : -1;
+            ownShift[cb] = a.lse[n];
+            ownTarget[cb] = (int32_t)a.target[n];
         }
-        if constexpr (PASS == kLossDt) {
-            if (biased) {
-                const float b = live ? a.bias[n] : -INFINITY;
-                live = b > kMaskedBelow;
-                ownShift[cb] = live ? b * kLog2e : -INFINITY;
-            }
+        if (kDt && SHIFT) {
+            ownShift[cb] = a.bias[n];
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            RowChunk<P> r;
-            r.clear();   // rows past the end, padding positions and free slots may hold anything
-            if (live) {
-                const int c = (ks * 2 + half) * 8;
-                r.load(static_cast<const char*>(a.own) + (n * a.ownStride * kElement + c * kElement), a.dim - c);
-            }
-            if (turned) {
-                r.negate();
-            }
-            r.planes(own[cb][ks], ownScale);
+            const int c = (ks * 2 + half) * 8;
+            ownRaw[cb][ks].clear();
+            ownRaw[cb][ks].load(static_cast<const char*>(a.own) + (n * a.ownStride * kElement + c * kElement), a.dim - c);
         }
     }
 
@@ -392,6 +366,8 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
     const int chunkCols = a.dim - chunk * 8;
     const int64_t strideBytes = a.streamStride * kElement;
     const uint32_t chunkAt = (uint32_t)(chunkRow * strideBytes + chunk * RowChunk<P>::kBytes);
+    float ownScale = 1.0f;
+    float streamScale = 1.0f;
     RowChunk<P> staged[L::kLoads];
 #pragma unroll
     for (int q = 0; q < L::kLoads; ++q) {
@@ -511,6 +487,52 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
             }
         }
     };
+
+    // ---- the first tile's loads, then the scales and the owners' planes ----
+    Aux next = aux_load(t0);   // of the tile that is placed next
+    Aux second = aux_load(t0 + 1);
+    fetch(t0);
+    // the forward pass bounds scores by the largest product, so there a negative scale goes into the owner's rows
+    const bool turned = PASS == kLossForward && a.scale < 0.0f;
+    float c2 = (turned ? -a.scale : a.scale) * kLog2e;
+    if constexpr (P == 2) {
+        float* largest = &auxA[0][0];   // free until the first tile is placed
+        const float o = wave_max(ownMost);
+        const float s = wave_max(streamMost);
+        if (lane == 0) {
+            largest[wave] = o;
+            largest[4 + wave] = s;
+        }
+        __syncthreads();
+        ownScale = plane_scale(fmaxf(fmaxf(largest[0], largest[1]), fmaxf(largest[2], largest[3])));
+        streamScale = plane_scale(fmaxf(fmaxf(largest[4], largest[5]), fmaxf(largest[6], largest[7])));
+        __syncthreads();
+        c2 = c2 / ownScale / streamScale;
+    }
+    Frag<P> own[CB][KS][P];
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        bool live = ownBase + cb * 32 + col < a.owners;
+        if constexpr (PASS == kLossDx) {
+            live = live && ownShift[cb] != INFINITY;
+            ownShift[cb] = live ? ownShift[cb] * kLog2e : INFINITY;
+            ownTarget[cb] = live ? ownTarget[cb] : -1;
+        }
+        if (kDt && SHIFT) {
+            live = live && ownShift[cb] > kMaskedBelow;
+            ownShift[cb] = live ? ownShift[cb] * kLog2e : -INFINITY;
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            if (!live) {
+                ownRaw[cb][ks].clear();   // rows past the end, padding positions and free slots may hold anything
+            }
+            if (turned) {
+                ownRaw[cb][ks].negate();
+            }
+            ownRaw[cb][ks].planes(own[cb][ks], ownScale);
+        }
+    }
 
     float top[CB];
     float sum[CB];
@@ -739,7 +761,6 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
         }
     };
 
-    Aux next = aux_load(t0);   // of the tile that is placed next
     auto sweep = [&](auto shiftedC, int from, int to) {
 #pragma unroll 1
         for (int t = from; t < to; ++t) {
@@ -766,22 +787,18 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
             __syncthreads();
         }
     };
-    if (t0 < t1) {
-        Aux second = aux_load(t0 + 1);
-        fetch(t0);
-        aux_mark(next, t0);
-        aux_mark(second, t0 + 1);
-        __syncthreads();
-        place(0, t0, next);
-        next = second;
-        __syncthreads();
-        if constexpr (SHIFT || kDt) {
-            sweep(std::integral_constant<bool, SHIFT>{}, t0, t1);
-        } else {
-            const int whole = max(t0, min(t1, a.streams / TR));
-            sweep(std::false_type{}, t0, whole);
-            sweep(std::true_type{}, whole, t1);
-        }
+    aux_mark(next, t0);
+    aux_mark(second, t0 + 1);
+    __syncthreads();
+    place(0, t0, next);
+    next = second;
+    __syncthreads();
+    if constexpr (SHIFT || kDt) {
+        sweep(std::integral_constant<bool, SHIFT>{}, t0, t1);
+    } else {
+        const int whole = max(t0, min(t1, a.streams / TR));
+        sweep(std::false_type{}, t0, whole);
+        sweep(std::true_type{}, whole, t1);
     }
     if (ownBase >= a.owners) {
         return;
