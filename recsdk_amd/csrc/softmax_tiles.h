@@ -624,6 +624,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
             }
         } else {
             Frag<P> g[CB][2][P];
+            bool hit = false;   // the piece holds a target of the wave's rows
             if constexpr (PASS == kLossDx) {
                 float b[16];
                 if constexpr (shifted) {
@@ -646,6 +647,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                     }
                     int d = ownTarget[cb] - rowBase;
                     if (__any((unsigned)d < 32u)) {
+                        hit = true;
                         d -= half;   // tile_row of a matrix row with 4 half in it
                         pin(d);
 #pragma unroll
@@ -665,7 +667,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                         shift[4 * q + j] = v[j];
                     }
                 }
-                const bool hit = __any((unsigned)(auxT[buf][r0 + col] - ownBase) < (unsigned)RW);
+                hit = __any((unsigned)(auxT[buf][r0 + col] - ownBase) < (unsigned)RW);
                 const uint32_t minus = __builtin_amdgcn_readfirstlane(minusBits[buf][r0 / 32]);
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
@@ -727,34 +729,52 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                     }
                 }
             }
-#pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    split_planes<P>(s[cb][i], i % 8, g[cb][i / 8]);
-                }
-            }
-            // second product: contracted over the piece's rows, in the order in which the registers hold them
+            // Second product: contracted over the piece's rows, in the order in which the registers hold them.  bfloat16: where the
+            // piece holds a target, whose value is nearly the whole gradient of its row, a second round adds what the rounding
+            // of the values has left, so that most gradients are off by their own rounding alone.  (A loop, not a branch with
+            // the product in it a second time: that made the compiler keep the accumulators twice.)
             const E* columnAt = &tile[buf][(r0 + 4 * ((lane & 15) >> 2) + half) * L::kRow + ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
+            bool again = P == 1 && hit;
+#pragma unroll 1
+            while (true) {
 #pragma unroll
-            for (int db = 0; db < DB; ++db) {
+                for (int cb = 0; cb < CB; ++cb) {
 #pragma unroll
-                for (int kk = 0; kk < 2; ++kk) {
-                    Frag<P> w[P];
-#pragma unroll
-                    for (int k = 0; k < P; ++k) {
-                        Short4 v[2];
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            const E* p = columnAt + k * L::kPlane + (16 * kk + 2 * j) * L::kRow + db * 32;
-                            v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                (__attribute__((address_space(3))) Short4*)(const_cast<E*>(p)));
-                        }
-                        __builtin_memcpy(&w[k], v, 16);
+                    for (int i = 0; i < 16; ++i) {
+                        split_planes<P>(s[cb][i], i % 8, g[cb][i / 8]);
                     }
+                }
 #pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) {
-                        acc[cb][db] = product<P>(w, g[cb][kk], acc[cb][db]);
+                for (int db = 0; db < DB; ++db) {
+#pragma unroll
+                    for (int kk = 0; kk < 2; ++kk) {
+                        Frag<P> w[P];
+#pragma unroll
+                        for (int k = 0; k < P; ++k) {
+                            Short4 v[2];
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const E* p = columnAt + k * L::kPlane + (16 * kk + 2 * j) * L::kRow + db * 32;
+                                v[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (__attribute__((address_space(3))) Short4*)(const_cast<E*>(p)));
+                            }
+                            __builtin_memcpy(&w[k], v, 16);
+                        }
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb) {
+                            acc[cb][db] = product<P>(w, g[cb][kk], acc[cb][db]);
+                        }
+                    }
+                }
+                if (!again) {
+                    break;
+                }
+                again = false;
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        s[cb][i] -= (float)(E)s[cb][i];
                     }
                 }
             }
