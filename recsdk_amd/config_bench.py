@@ -1,7 +1,7 @@
 """Throughput of the hot path on the synthetic configurations other than the headline one (which bench.py measures):
 keys/s and algorithmic GB/s, as a fraction of the 8 TB/s HBM peak.  One JSON line per configuration.
 
-    python -m recsdk_amd.config_bench --config c1|c3|c4|c5|ops|keys|bounds|all [--steps K] [--warmup W]
+    python -m recsdk_amd.config_bench --config c1|c3|c4|c5|ops|keys|head|bounds|all [--steps K] [--warmup W]
 
   c1  one fp32 table 1M x 16, batch 4096 uniform keys, forward gather + sparse Adagrad
   c3  26 bf16 tables 2M x 64, batch 16384, bag lengths U[1,50], Zipf(1.1): sum-pooled forward + exact backward + Adam
@@ -9,6 +9,9 @@ keys/s and algorithmic GB/s, as a fraction of the 8 TB/s HBM peak.  One JSON lin
       admission at count >= 2, eviction of keys idle > 20 steps, gather + Adam on the admitted keys
   ops the by-address lookup / update operators and the fused LazyAdam / Sgd operators one by one, 512-byte rows
   keys batch ingestion, padding mask, sharded unique, sorted unique and hot-key split on 26 x 65536 Zipf(1.05) keys
+  head the training head behind a pooled lookup, through the torch operators with autograd: bags of a 2M x 64 bf16 table,
+      dropout, layer norm, softmax loss over an item table of 200k x 64 bf16 with popularity corrections, and the gradient
+      back into both tables
   bounds the drop-in libraries (AccCTR plugin, Embcache classes) called with host vectors, beside the CPU restatement
   c5  host-backed cache: dim 64 rows in pinned host DRAM behind a 20M-row HBM cache, batch 65536 x 26 keys Zipf(1.05):
       unique, cache plan, swap-out / swap-in, gather + Adagrad.  --host-rows scales the host table (default 100M rows
@@ -307,6 +310,74 @@ def run_c3(args, torch, capi, host, synth):
     elapsed = _timed(torch, step_unique, args.warmup, args.steps)
     _line("C3", "the same step with unique_ids / unique_offsets / unique_inverse given (the reference's unique backward)",
           nnz, nbytes + nnz * 8 + uniq * 8, args.steps, elapsed, dict(c3_extra))
+
+
+def run_head(args, torch, capi, host, synth):
+    """One training step of a retrieval model around this library's operators: pooled lookup of each user's items, dropout,
+    layer norm, softmax loss over the item table; backward through the loss, the norm, the dropout and into the lookup's
+    fused Adam; the item table's gradient is dense.  Also the three operators of the head by themselves, forward and
+    backward.  Bytes: each operand and result once; the loss is bound by its products (6 rows items dim with the scores
+    kept), reported as TFLOP/s."""
+    from . import torch_ops
+    torch_ops.load()
+    fbgemm, ops = torch.ops.fbgemm, torch.ops.recsdk
+    dev = "cuda:0"
+    B, D, rows, items, nb = 8192, 64, 2_000_000, 200_000, 3
+    rng = np.random.default_rng(0)
+    batches = []
+    for _ in range(nb):
+        offsets = np.concatenate([[0], np.cumsum(rng.integers(1, 51, B))]).astype(np.int64)
+        idx = synth.zipf_ranks(rng, 1.1, rows, int(offsets[-1])).astype(np.int64)
+        target = synth.zipf_ranks(rng, 1.1, items, B).astype(np.int64)
+        target[rng.random(B) < 0.05] = -1                      # keys that were not admitted
+        batches.append(tuple(torch.from_numpy(a).to(dev) for a in (idx, offsets, target)))
+    w = (torch.randn(rows * D, device=dev) * 0.01).to(torch.bfloat16)
+    m1, m2 = torch.zeros(rows * D, device=dev), torch.zeros(rows * D, device=dev)
+    table = (torch.randn(items, D, device=dev) * 0.1).to(torch.bfloat16).requires_grad_()
+    item_bias = torch.log1p(torch.arange(items, device=dev, dtype=torch.float32))   # minus the log of a Zipf item's share
+    weight, bias = torch.ones(D, device=dev, requires_grad=True), torch.zeros(D, device=dev, requires_grad=True)
+    none = torch.empty(0, device=dev)
+    leaf = torch.zeros(1, device=dev, requires_grad=True)
+    woff = torch.zeros(1, device=dev, dtype=torch.int64)
+    doff = torch.tensor([0, D], device=dev, dtype=torch.int32)
+    hcs = torch.tensor([0, rows], device=dev, dtype=torch.int64)
+
+    def loss_of(x, target, i):
+        x = ops.dropout(x, 0.1, 17, i)
+        x = ops.layer_norm(x, weight, bias)
+        return ops.softmax_loss(x.to(torch.bfloat16), table, target, item_bias, 1.0 / 8).sum() / B
+
+    def step(i):
+        idx, offs, target = batches[i % nb]
+        pooled = fbgemm.split_embedding_codegen_lookup_adam_function(
+            leaf, w, none, none, none, woff, doff, D, D, hcs, 21, idx, offs, capi.POOL_MEAN, None, None, none, False, 0.0, False,
+            m1, none, none, none, m2, none, none, none, eps=1e-8, learning_rate=1e-3, beta1=0.9, beta2=0.999, iter=i + 1)
+        for t in (table, weight, bias):
+            t.grad = None
+        loss_of(pooled, target, i).backward()
+
+    nnz = float(np.mean([int(b[0].numel()) for b in batches]))
+    flops = 6.0 * B * items * D
+    nbytes = 20 * nnz + 2 * 2 * items * D + 3 * 4 * B * D * 4
+
+    def line(name, elapsed):
+        ms = elapsed / args.steps * 1e3
+        tf = flops / ms / 1e9
+        _line("HEAD", name, nnz, nbytes, args.steps, elapsed,
+              {"TFLOPs": round(tf, 1), "roofline": {"bound": "mfma", "scope": "whole step", "achieved": round(tf, 1), "peak": 2500.0,
+                                                    "unit": "TFLOP/s", "frac": round(tf / 2500.0, 4), "traffic": None}})
+
+    line("pooled lookup 2M x 64 bf16, batch 8192, bags U[1,50], dropout, layer norm, softmax loss over 200k x 64 bf16 items; "
+         "backward into both tables", _timed(torch, step, args.warmup, args.steps))
+    x = torch.randn(B, D, device=dev, requires_grad=True)
+
+    def head_only(i):
+        for t in (x, table, weight, bias):
+            t.grad = None
+        loss_of(x, batches[i % nb][2], i).backward()
+
+    line("the head alone: dropout, layer norm, softmax loss over 200k x 64 bf16 items, forward and backward",
+         _timed(torch, head_only, args.warmup, args.steps))
 
 
 def run_c4(args, torch, capi, host, synth):
@@ -708,7 +779,7 @@ def make_parser():
     """The command line of this module; `default_args` hands its defaults to callers that run a configuration
     in-process, so the two never drift apart."""
     ap = argparse.ArgumentParser()
-    ap.add_argument("--config", default="all", choices=["c1", "c3", "c4", "c5", "ops", "keys", "bounds", "all"])
+    ap.add_argument("--config", default="all", choices=["c1", "c3", "c4", "c5", "ops", "keys", "head", "bounds", "all"])
     ap.add_argument("--steps", type=int, default=None, help="timed steps (default 20; c4: 100, as the configuration says)")
     ap.add_argument("--two-stages", action="store_true",
                     help="c5: dedup, plan and move of the next batch on ONE second stream (default: three stages)")
@@ -754,7 +825,7 @@ def main():
 
     capi.lib()
     torch.cuda.set_device(0)
-    runs = {"c1": run_c1, "c3": run_c3, "c4": run_c4, "c5": run_c5, "ops": run_ops, "keys": run_keys,
+    runs = {"c1": run_c1, "c3": run_c3, "c4": run_c4, "c5": run_c5, "ops": run_ops, "keys": run_keys, "head": run_head,
             "bounds": run_bounds}
     steps = args.steps
     warmup = args.warmup

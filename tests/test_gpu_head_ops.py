@@ -584,6 +584,36 @@ def test_lookup_dropout_norm_loss_and_table_update(ops):
         assert (got.detach().double().cpu() - want).abs().max() <= 2e-5 * want.abs().max()
 
 
+def test_head_configuration_of_the_benchmark_runs(capsys):
+    import json
+
+    from recsdk_amd import config_bench as cb
+    from recsdk_amd import synth
+
+    cb.run_head(cb.default_args(config="head", steps=2, warmup=1), torch, capi, host, synth)
+    lines = [json.loads(text) for text in capsys.readouterr().out.splitlines() if text.startswith("{")]
+    assert len(lines) == 2 and all(d["config"] == "HEAD" and d["TFLOPs"] > 0 for d in lines)
+
+
+@pytest.mark.parametrize("each", [1.015, 1.0, 0.6])
+def test_bfloat16_gradients_are_off_by_their_own_rounding(ops, each):
+    """Rows of equal weight, just above a power of two, where the rounding of the values would weigh most: the gradients' error
+    stays near what rounding the exact gradients alone leaves."""
+    x, table, target, _ = loss_case(256, 20000, 64, "bf16", 81)
+    grad = torch.full((256,), each / 256, device=DEV)
+    leaves = [t.detach().requires_grad_() for t in (x, table)]
+    got = torch.autograd.grad(ops.softmax_loss(*leaves, target, None, 0.3), leaves, grad)
+    z = 0.3 * x.double() @ table.double().t()
+    q = torch.softmax(z, 1)
+    q[torch.arange(256, device=DEV), target] -= 1
+    q *= 0.3 * each / 256
+    for a, exact in zip(got, (q @ table.double(), q.t() @ x.double())):
+        own = (exact.bfloat16().double() - exact).norm()
+        # beside the targets' terms (2^-16 after two rounds) the other probabilities, 2^-8 off at most, make up a few percent of
+        # the gradients of x and less of the table's
+        assert (a.double() - exact).norm() <= 1.15 * own
+
+
 # ---- refusals that need a device -------------------------------------------------------------------------------------
 
 def test_refusals_of_the_torch_operators(ops):
