@@ -744,7 +744,7 @@ RECSDK_API int recsdk_dropout(const void* d_x, int64_t n, int32_t dtype, double 
  *   dtype      of x and y: RECSDK_DT_F32, RECSDK_DT_F16 or RECSDK_DT_BF16; w_dtype of weight and bias: dtype or RECSDK_DT_F32
  *   x_stride   elements between rows of x (>= dim); y is contiguous and does not overlap x
  *   d_weight, d_bias   [dim] or NULL (1 and 0);  d_mean, d_rstd  [rows] fp32 for the backward pass, or both NULL
- * Statistics and sums are fp32.  Any dim; rows < 2^31. */
+ * Statistics and sums are fp32.  dim < 2^30, rows < 2^31. */
 RECSDK_API int recsdk_layer_norm_forward(const void* d_x, int64_t rows, int32_t dim, int64_t x_stride, int32_t dtype,
                                          const void* d_weight, const void* d_bias, int32_t w_dtype, float eps, void* d_y,
                                          float* d_mean, float* d_rstd, void* stream);
@@ -767,8 +767,13 @@ RECSDK_API int recsdk_layer_norm_backward(const void* d_grad, const void* d_x, i
  *                  item out: a free slot of the table, whose row may hold anything.  A row whose target is taken out
  *                  (so also one that no item is left for) has loss +infinity and gives no gradient
  *   d_loss, d_lse  [rows] fp32; d_lse is for the backward pass: log-sum-exp, or +infinity where a row gives no gradient
- * d_x, d_table, d_workspace, and the gradients d_dx and d_dtable are 16-byte aligned.  Sums and statistics are fp32; bf16 probabilities are rounded to bf16
- * where they enter the gradients' products.  rows and items < 2^30, items >= 1. */
+ *   scale          any finite value
+ * d_x, d_table, d_workspace, and the gradients d_dx and d_dtable are 16-byte aligned.  rows and items < 2^30, items >= 1.
+ * Rows that are no whole 16-byte pieces, or more than 2^22 elements apart, are copied into the workspace first.
+ * Sums and statistics are fp32.  The gradients take (probability - [target]) grad in the operands' precision: bf16 in one
+ * rounding, and a second one of what the first has left where a target is among 32 rows at a time.  fp32 products of more
+ * than 32 rows keep 22 bits of each value, and of an operand nothing below 2^-40 of its largest finite one, in rows and items that
+ * take part; an infinity in one of those rows or items counts as NaN.  Products of up to 32 rows keep 24 bits. */
 RECSDK_API int recsdk_softmax_loss_workspace(int64_t rows, int64_t items, int32_t dim, int32_t dtype, int64_t x_stride,
                                              int64_t table_stride, int64_t* h_forward_bytes, int64_t* h_backward_bytes);
 RECSDK_API int recsdk_softmax_loss_forward(const void* d_x, int64_t rows, int64_t x_stride, const void* d_table, int64_t items,

@@ -74,7 +74,8 @@ __device__ __forceinline__ void store_columns(T* row, int d, int dim, bool fours
     typedef T T4 __attribute__((ext_vector_type(4)));
     if (fours) {
         if (d < dim) {
-            *reinterpret_cast<T4*>(row + d) = T4{from_float<T>(v[0]), from_float<T>(v[1]), from_float<T>(v[2]), from_float<T>(v[3])};
+            *reinterpret_cast<T4*>(row + d) =
+                T4{from_float<T>(v[0]), from_float<T>(v[1]), from_float<T>(v[2]), from_float<T>(v[3])};
         }
     } else {
 #pragma unroll

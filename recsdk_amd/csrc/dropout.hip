@@ -153,7 +153,7 @@ static int launch_dropout(const void* x, void* y, int64_t n, uint32_t below, flo
 {
     const bool whole = aligned16(x) && aligned16(y);
     const int64_t grid = whole ? cdiv(n, (int64_t)kBlock * kDropItems * (16 / (int)sizeof(T))) : cdiv(cdiv(n, 8), kBlock);
-    RECSDK_REQUIRE(grid < (int64_t(1) << 31), RECSDK_EINVAL, "recsdk_dropout: too large for one launch");
+    RECSDK_REQUIRE(grid * kBlock < (int64_t(1) << 32), RECSDK_EINVAL, "recsdk_dropout: too large for one launch");
     const T* px = static_cast<const T*>(x);
     T* py = static_cast<T*>(y);
     if (whole) {

@@ -25,6 +25,7 @@ constexpr int kNormBlocks = 1024;       // blocks of the backward pass at most: 
 constexpr int kNormRowBlocks = 512;     // of them, where a block holds few rows' worth of registers
 constexpr int kNormForwardBlocks = 2048;
 constexpr int kNormSpanBlocks = 2048;
+constexpr int kNormWideBlocks = 65536;  // a launch holds fewer than 2^32 threads
 constexpr int kSpanBytes = 16384;       // rows that a block stages at once
 constexpr int kSpanLoads = kSpanBytes / 16 / kBlock;
 constexpr int kSpanRows = kBlock;       // at most: one thread fetches a row's statistics
@@ -640,29 +641,31 @@ template <typename T, typename W>
 __global__ __launch_bounds__(1024) void k_layer_norm_wide(NormRows a)
 {
     __shared__ float smem[32];
-    const T* x = static_cast<const T*>(a.x) + (int64_t)blockIdx.x * a.stride;
-    T* y = static_cast<T*>(a.y) + (int64_t)blockIdx.x * a.dim;
     const float inv = 1.0f / (float)a.dim;
-    float sum[1] = {0.0f};
-    for (int c = threadIdx.x; c < a.dim; c += 1024) {
-        sum[0] += (float)x[c];
-    }
-    team_sum<1024>(sum, smem);
-    const float mean = sum[0] * inv;
-    sum[0] = 0.0f;
-    for (int c = threadIdx.x; c < a.dim; c += 1024) {
-        const float d = (float)x[c] - mean;
-        sum[0] = __builtin_fmaf(d, d, sum[0]);
-    }
-    team_sum<1024>(sum, smem);
-    const float rstd = 1.0f / sqrtf(sum[0] * inv + a.eps);
-    for (int c = threadIdx.x; c < a.dim; c += 1024) {
-        y[c] = from_float<T>(__builtin_fmaf(((float)x[c] - mean) * rstd, param<W>(a.weight, c, 1.0f),
-                                            param<W>(a.bias, c, 0.0f)));
-    }
-    if (threadIdx.x == 0 && a.mean != nullptr) {
-        a.mean[blockIdx.x] = mean;
-        a.rstd[blockIdx.x] = rstd;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.stride;
+        T* y = static_cast<T*>(a.y) + row * a.dim;
+        float sum[1] = {0.0f};
+        for (int c = threadIdx.x; c < a.dim; c += 1024) {
+            sum[0] += (float)x[c];
+        }
+        team_sum<1024>(sum, smem);
+        const float mean = sum[0] * inv;
+        sum[0] = 0.0f;
+        for (int c = threadIdx.x; c < a.dim; c += 1024) {
+            const float d = (float)x[c] - mean;
+            sum[0] = __builtin_fmaf(d, d, sum[0]);
+        }
+        team_sum<1024>(sum, smem);
+        const float rstd = 1.0f / sqrtf(sum[0] * inv + a.eps);
+        for (int c = threadIdx.x; c < a.dim; c += 1024) {
+            y[c] = from_float<T>(__builtin_fmaf(((float)x[c] - mean) * rstd, param<W>(a.weight, c, 1.0f),
+                                                param<W>(a.bias, c, 0.0f)));
+        }
+        if (threadIdx.x == 0 && a.mean != nullptr) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
     }
 }
 
@@ -670,23 +673,25 @@ template <typename T, typename W>
 __global__ __launch_bounds__(1024) void k_layer_norm_wide_dx(NormRows a)
 {
     __shared__ float smem[32];
-    const T* x = static_cast<const T*>(a.x) + (int64_t)blockIdx.x * a.stride;
-    const T* dy = static_cast<const T*>(a.grad) + (int64_t)blockIdx.x * a.dim;
-    T* dx = static_cast<T*>(a.dx) + (int64_t)blockIdx.x * a.dim;
-    const float mean = a.mean[blockIdx.x];
-    const float rstd = a.rstd[blockIdx.x];
-    float s[2] = {0.0f, 0.0f};
-    for (int c = threadIdx.x; c < a.dim; c += 1024) {
-        const float g = (float)dy[c] * param<W>(a.weight, c, 1.0f);
-        s[0] += g;
-        s[1] = __builtin_fmaf(g, ((float)x[c] - mean) * rstd, s[1]);
-    }
-    team_sum<1024>(s, smem);
-    const float s0 = s[0] / (float)a.dim;
-    const float s1 = s[1] / (float)a.dim;
-    for (int c = threadIdx.x; c < a.dim; c += 1024) {
-        const float g = (float)dy[c] * param<W>(a.weight, c, 1.0f);
-        dx[c] = from_float<T>(rstd * (g - s0 - ((float)x[c] - mean) * rstd * s1));
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.stride;
+        const T* dy = static_cast<const T*>(a.grad) + row * a.dim;
+        T* dx = static_cast<T*>(a.dx) + row * a.dim;
+        const float mean = a.mean[row];
+        const float rstd = a.rstd[row];
+        float s[2] = {0.0f, 0.0f};
+        for (int c = threadIdx.x; c < a.dim; c += 1024) {
+            const float g = (float)dy[c] * param<W>(a.weight, c, 1.0f);
+            s[0] += g;
+            s[1] = __builtin_fmaf(g, ((float)x[c] - mean) * rstd, s[1]);
+        }
+        team_sum<1024>(s, smem);
+        const float s0 = s[0] / (float)a.dim;
+        const float s1 = s[1] / (float)a.dim;
+        for (int c = threadIdx.x; c < a.dim; c += 1024) {
+            const float g = (float)dy[c] * param<W>(a.weight, c, 1.0f);
+            dx[c] = from_float<T>(rstd * (g - s0 - ((float)x[c] - mean) * rstd * s1));
+        }
     }
 }
 
@@ -867,9 +872,10 @@ static int launch_staged(const NormRows& a, int* blocks, hipStream_t stream)
 template <typename T, typename W, bool BACK>
 static int launch_wide(const NormRows& a, int* blocks, hipStream_t stream)
 {
+    const dim3 grid((unsigned)(a.rows < kNormWideBlocks ? a.rows : kNormWideBlocks));
     if constexpr (BACK) {
         if (a.dx != nullptr) {
-            RECSDK_LAUNCH_AS("k_layer_norm_wide_dx", (k_layer_norm_wide_dx<T, W>), dim3((unsigned)a.rows), dim3(1024), stream, a);
+            RECSDK_LAUNCH_AS("k_layer_norm_wide_dx", (k_layer_norm_wide_dx<T, W>), grid, dim3(1024), stream, a);
         }
         if (a.part != nullptr) {
             *blocks = norm_backward_blocks(a.rows, 16, kNormBlocks);
@@ -877,7 +883,7 @@ static int launch_wide(const NormRows& a, int* blocks, hipStream_t stream)
                              dim3((unsigned)cdiv(a.dim, kBlock), (unsigned)*blocks), dim3(kBlock), stream, a);
         }
     } else {
-        RECSDK_LAUNCH_AS("k_layer_norm_wide", (k_layer_norm_wide<T, W>), dim3((unsigned)a.rows), dim3(1024), stream, a);
+        RECSDK_LAUNCH_AS("k_layer_norm_wide", (k_layer_norm_wide<T, W>), grid, dim3(1024), stream, a);
     }
     return RECSDK_OK;
 }
@@ -941,8 +947,8 @@ static int check_norm(const char* name, int64_t rows, int32_t dim, int64_t x_str
         set_error("%s: weight and bias must be fp32 or of the rows' type", name);
         return RECSDK_EINVAL;
     }
-    if (dim < 1 || rows < 0 || rows >= (int64_t(1) << 31)) {
-        set_error("%s: dim must be at least 1 and rows below 2^31", name);
+    if (dim < 1 || dim >= (1 << 30) || rows < 0 || rows >= (int64_t(1) << 31)) {
+        set_error("%s: dim must lie in [1, 2^30) and rows in [0, 2^31)", name);
         return RECSDK_EINVAL;
     }
     if (x_stride < dim) {
@@ -988,7 +994,7 @@ extern "C" int recsdk_layer_norm_workspace(int64_t rows, int32_t dim, int64_t* h
 {
     using namespace recsdk;
     RECSDK_REQUIRE(h_bytes != nullptr, RECSDK_ENULL, "recsdk_layer_norm_workspace: NULL argument");
-    RECSDK_REQUIRE(rows >= 0 && dim >= 1, RECSDK_EINVAL, "recsdk_layer_norm_workspace: bad sizes");
+    RECSDK_REQUIRE(rows >= 0 && dim >= 1 && dim < (1 << 30), RECSDK_EINVAL, "recsdk_layer_norm_workspace: bad sizes");
     *h_bytes = (int64_t)norm_backward_blocks(rows, 1, kNormBlocks) * 2 * dim * (int64_t)sizeof(float);
     return RECSDK_OK;
 }

@@ -1,11 +1,14 @@
 // The softmax loss's entry points and the kernels around the tile kernels (softmax_tiles.h, where the method stands): joins of
 // partial results, padded copies, largest values.
+#include <algorithm>
+
 #include "softmax_tiles.h"
 
 namespace recsdk {
 
 constexpr int kFewRows = 32;
 constexpr int kAbsMaxThreads = 1024;
+constexpr int64_t kMostBlocks = 65536;   // of the kernels here, which walk what is more: a launch holds fewer than 2^32 threads
 
 // Joins the parts of the running sums and takes the target's score off.  TEAM threads per row of x: a wave, or the block
 // where there are few rows, each with many parts.
@@ -18,61 +21,61 @@ __global__ __launch_bounds__(kBlock) void k_softmax_loss_join(const float2* __re
 {
     constexpr int kWaves = TEAM / kWave;
     __shared__ float joined[kWaves][2];
-    const int n = blockIdx.x * (kBlock / TEAM) + threadIdx.x / TEAM;
     const int lane = threadIdx.x % TEAM;
-    if (n >= rows) {
-        return;
-    }
-    const int64_t t = target[n];
-    const bool inside = t >= 0 && t < items;
-    const float b = inside && bias != nullptr ? bias[t] : 0.0f;
-    if (!inside || b <= kMaskedBelow) {
-        // no target: no loss; a target that is taken out: infinite; neither gives a gradient
-        if (lane == 0) {
-            loss[n] = inside ? INFINITY : 0.0f;
-            lse[n] = INFINITY;
+    for (int64_t n = (int64_t)blockIdx.x * (kBlock / TEAM) + threadIdx.x / TEAM; n < rows;
+         n += (int64_t)gridDim.x * (kBlock / TEAM)) {
+        const int64_t t = target[n];
+        const bool inside = t >= 0 && t < items;
+        const float b = inside && bias != nullptr ? bias[t] : 0.0f;
+        if (!inside || b <= kMaskedBelow) {
+            // no target: no loss; a target that is taken out: infinite; neither gives a gradient
+            if (lane == 0) {
+                loss[n] = inside ? INFINITY : 0.0f;
+                lse[n] = INFINITY;
+            }
+            continue;   // the whole team
         }
-        return;   // the whole team
-    }
-    float dot = 0.0f;
-    for (int d = lane; d < dim && lane < kWave; d += kWave) {
-        dot = __builtin_fmaf((float)x[n * xStride + d], (float)table[t * tableStride + d], dot);
-    }
-    float top = kFloor;
-    float sum = 0.0f;
+        float dot = 0.0f;
+        for (int d = lane; d < dim && lane < kWave; d += kWave) {
+            dot = __builtin_fmaf((float)x[n * xStride + d], (float)table[t * tableStride + d], dot);
+        }
+        float top = kFloor;
+        float sum = 0.0f;
 #pragma unroll 4
-    for (int p = lane; p < parts; p += TEAM) {
-        const float2 v = norm[(int64_t)p * rows + n];
-        const float now = fmaxf(top, v.x);
-        sum = sum * exp2_fast(top - now) + v.y * exp2_fast(v.x - now);
-        top = now;
-    }
-#pragma unroll
-    for (int d = kWave / 2; d > 0; d >>= 1) {
-        const float otherTop = __shfl_xor(top, d, kWave);
-        const float otherSum = __shfl_xor(sum, d, kWave);
-        const float now = fmaxf(top, otherTop);
-        sum = sum * exp2_fast(top - now) + otherSum * exp2_fast(otherTop - now);
-        top = now;
-        dot += __shfl_xor(dot, d, kWave);
-    }
-    if constexpr (kWaves > 1) {
-        if (lane % kWave == 0) {
-            joined[lane / kWave][0] = top;
-            joined[lane / kWave][1] = sum;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int w = 1; w < kWaves; ++w) {
-            const float now = fmaxf(top, joined[w][0]);
-            sum = sum * exp2_fast(top - now) + joined[w][1] * exp2_fast(joined[w][0] - now);
+        for (int p = lane; p < parts; p += TEAM) {
+            const float2 v = norm[(int64_t)p * rows + n];
+            const float now = fmaxf(top, v.x);
+            sum = sum * exp2_fast(top - now) + v.y * exp2_fast(v.x - now);
             top = now;
         }
-    }
-    if (lane == 0) {
-        const float l = __builtin_fmaf(top, kLn2, logf(sum));
-        loss[n] = l - __builtin_fmaf(dot, scale, b);
-        lse[n] = l;
+#pragma unroll
+        for (int d = kWave / 2; d > 0; d >>= 1) {
+            const float otherTop = __shfl_xor(top, d, kWave);
+            const float otherSum = __shfl_xor(sum, d, kWave);
+            const float now = fmaxf(top, otherTop);
+            sum = sum * exp2_fast(top - now) + otherSum * exp2_fast(otherTop - now);
+            top = now;
+            dot += __shfl_xor(dot, d, kWave);
+        }
+        if constexpr (kWaves > 1) {
+            __syncthreads();   // the previous row's have been read
+            if (lane % kWave == 0) {
+                joined[lane / kWave][0] = top;
+                joined[lane / kWave][1] = sum;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int w = 1; w < kWaves; ++w) {
+                const float now = fmaxf(top, joined[w][0]);
+                sum = sum * exp2_fast(top - now) + joined[w][1] * exp2_fast(joined[w][0] - now);
+                top = now;
+            }
+        }
+        if (lane == 0) {
+            const float l = __builtin_fmaf(top, kLn2, logf(sum));
+            loss[n] = l - __builtin_fmaf(dot, scale, b);
+            lse[n] = l;
+        }
     }
 }
 
@@ -88,38 +91,41 @@ __global__ __launch_bounds__(kBlock) void k_softmax_grad_join(const float* __res
     __shared__ Float4 sums[WAYS > 1 ? WAYS : 1][WAYS > 1 ? kWide : 1];
     const int way = threadIdx.x / kWide;
     const int at = threadIdx.x % kWide;
-    const int64_t i = ((int64_t)blockIdx.x * kWide + at) * 4;
-    Float4 s = 0.0f;
-    if (i < count) {
+    for (int64_t block = blockIdx.x; block * kWide * 4 < count; block += gridDim.x) {
+        const int64_t i = (block * kWide + at) * 4;
+        Float4 s = 0.0f;
+        if (i < count) {
 #pragma unroll 8
-        for (int p = way; p < parts; p += WAYS) {
-            s += *reinterpret_cast<const Float4*>(part + p * count + i);
+            for (int p = way; p < parts; p += WAYS) {
+                s += *reinterpret_cast<const Float4*>(part + p * count + i);
+            }
         }
-    }
-    if constexpr (WAYS > 1) {
-        sums[way][at] = s;
-        __syncthreads();
-        if (way != 0) {
-            return;
-        }
+        if constexpr (WAYS > 1) {
+            __syncthreads();   // the previous block's sums have been read
+            sums[way][at] = s;
+            __syncthreads();
+            if (way != 0) {
+                continue;
+            }
 #pragma unroll
-        for (int w = 1; w < WAYS; ++w) {
-            s += sums[w][at];
+            for (int w = 1; w < WAYS; ++w) {
+                s += sums[w][at];
+            }
         }
-    }
-    if (i >= count) {
-        return;
-    }
-    const int64_t n = i / partDim;
-    float factor = 1.0f;
-    if (grad != nullptr) {
-        factor = grad[n] * scale;
-        if (lse[n] == INFINITY) {   // takes no gradient, whatever grad holds
-            s = 0.0f;
-            factor = 0.0f;
+        if (i >= count) {
+            continue;
         }
+        const int64_t n = i / partDim;
+        float factor = 1.0f;
+        if (grad != nullptr) {
+            factor = grad[n] * scale;
+            if (lse[n] == INFINITY) {   // takes no gradient, whatever grad holds
+                s = 0.0f;
+                factor = 0.0f;
+            }
+        }
+        store_columns(out + n * dim, (int)(i - n * partDim), dim, dim % 4 == 0, s * factor);
     }
-    store_columns(out + n * dim, (int)(i - n * partDim), dim, dim % 4 == 0, s * factor);
 }
 
 // Rows of `dim` elements at any stride -> rows of `padded` elements (whole 16-byte pieces), the rest zero.  32 threads take
@@ -129,17 +135,15 @@ __global__ __launch_bounds__(kBlock) void k_pad_rows(const T* __restrict__ src, 
                                                      T* __restrict__ dst)
 {
     constexpr int kPer = 16 / sizeof(T);
-    const int64_t r = (int64_t)blockIdx.x * (kBlock / 32) + threadIdx.x / 32;
-    if (r >= rows) {
-        return;
-    }
-    for (int c = threadIdx.x % 32 * kPer; c < padded; c += 32 * kPer) {
-        Pack<T, kPer> v;
+    for (int64_t r = (int64_t)blockIdx.x * (kBlock / 32) + threadIdx.x / 32; r < rows; r += (int64_t)gridDim.x * (kBlock / 32)) {
+        for (int c = threadIdx.x % 32 * kPer; c < padded; c += 32 * kPer) {
+            Pack<T, kPer> v;
 #pragma unroll
-        for (int e = 0; e < kPer; ++e) {
-            v.v[e] = c + e < dim ? src[r * stride + c + e] : from_float<T>(0.0f);
+            for (int e = 0; e < kPer; ++e) {
+                v.v[e] = c + e < dim ? src[r * stride + c + e] : from_float<T>(0.0f);
+            }
+            *reinterpret_cast<Pack<T, kPer>*>(dst + r * padded + c) = v;
         }
-        *reinterpret_cast<Pack<T, kPer>*>(dst + r * padded + c) = v;
     }
 }
 
@@ -231,7 +235,7 @@ struct LossPlan {
     int planes;
     int bytes;           // of an element
     int padded;          // columns of padded copies
-    bool padX;           // rows that are no whole 16-byte pieces are copied into padded ones first
+    bool padX;           // rows that are no whole 16-byte pieces, or too far apart, are copied into padded ones first
     bool padTable;
     PassPlan forward, dx, dt;
     int64_t atX, atTable, atMax, atParts;   // offsets into the workspace
@@ -247,8 +251,8 @@ static LossPlan plan_loss(int64_t rows, int64_t items, int32_t dim, int32_t dtyp
     p.bytes = float_bytes(dtype);
     const int piece = 16 / p.bytes;
     p.padded = (int)(cdiv(dim, piece) * piece);
-    p.padX = dim % piece != 0 || x_stride % piece != 0;
-    p.padTable = dim % piece != 0 || table_stride % piece != 0;
+    p.padX = dim % piece != 0 || x_stride % piece != 0 || x_stride > kLossMaxStride;
+    p.padTable = dim % piece != 0 || table_stride % piece != 0 || table_stride > kLossMaxStride;
     p.forward = plan_pass(p.planes, dim, rows, items, kLossForward);
     p.dx = plan_pass(p.planes, dim, rows, items, kLossDx);
     p.dt = plan_pass(p.planes, dim, items, rows, kLossDt);
@@ -294,10 +298,6 @@ static int check_loss(const char* name, int64_t rows, int64_t items, int32_t dim
         set_error("%s: rows overlap (stride < dim)", name);
         return RECSDK_EINVAL;
     }
-    if (x_stride > kLossMaxStride || table_stride > kLossMaxStride) {
-        set_error("%s: rows are more than %d elements apart", name, kLossMaxStride);
-        return RECSDK_EINVAL;
-    }
     return RECSDK_OK;
 }
 
@@ -305,7 +305,7 @@ static int check_loss(const char* name, int64_t rows, int64_t items, int32_t dim
 template <typename T>
 static int pad_operand(const void*& p, int64_t& stride, int64_t rows, int dim, int padded, void* to, hipStream_t stream)
 {
-    const int64_t grid = cdiv(rows, kBlock / 32);
+    const int64_t grid = std::min(cdiv(rows, kBlock / 32), kMostBlocks);
     RECSDK_LAUNCH_AS("k_pad_rows", (k_pad_rows<T>), dim3((unsigned)grid), dim3(kBlock), stream, static_cast<const T*>(p), stride,
                      rows, dim, padded, static_cast<T*>(to));
     p = to;
@@ -318,8 +318,7 @@ static int launch_grad_join(const float* part, int parts, int64_t rows, int dim,
                             float scale, void* out, hipStream_t stream)
 {
     const int partDim = (int)cdiv(dim, 4) * 4;
-    const int64_t grid = cdiv(rows * partDim, (int64_t)kBlock / WAYS * 4);
-    RECSDK_REQUIRE(grid < (int64_t(1) << 31), RECSDK_EINVAL, "softmax loss: table too large for one launch");
+    const int64_t grid = std::min(cdiv(rows * partDim, (int64_t)kBlock / WAYS * 4), kMostBlocks);
     RECSDK_LAUNCH_AS("k_softmax_grad_join", (k_softmax_grad_join<T, WAYS>), dim3((unsigned)grid), dim3(kBlock), stream, part,
                      parts, rows * partDim, dim, partDim, lse, grad, scale, static_cast<T*>(out));
     return RECSDK_OK;
@@ -362,9 +361,9 @@ static int find_largest(const LossPlan& plan, const LossOperands& o, int64_t row
                         const float* bias, char* workspace, hipStream_t stream)
 {
     if (plan.planes == 2) {
-        RECSDK_LAUNCH_AS("k_abs_max", k_abs_max, dim3(2 * kAbsMaxParts), dim3(kAbsMaxThreads), stream, static_cast<const float*>(o.x),
-                         o.xStride, (int)rows, static_cast<const float*>(o.table), o.tableStride, (int)items, dim, target, bias,
-                         reinterpret_cast<float*>(workspace + plan.atMax));
+        RECSDK_LAUNCH_AS("k_abs_max", k_abs_max, dim3(2 * kAbsMaxParts), dim3(kAbsMaxThreads), stream,
+                         static_cast<const float*>(o.x), o.xStride, (int)rows, static_cast<const float*>(o.table), o.tableStride,
+                         (int)items, dim, target, bias, reinterpret_cast<float*>(workspace + plan.atMax));
     }
     return RECSDK_OK;
 }
@@ -403,14 +402,17 @@ static int run_forward(const LossPlan& plan, LossOperands o, int64_t rows, int64
     }
     const T* x = static_cast<const T*>(given.x);
     const T* table = static_cast<const T*>(given.table);
-    if (plan.forward.parts >= 4 * kWave) {
-        RECSDK_LAUNCH_AS("k_softmax_loss_join", (k_softmax_loss_join<T, kBlock>), dim3((unsigned)rows), dim3(kBlock), stream,
-                         a.norm, plan.forward.parts, (int)rows, (int)items, dim, x, given.xStride, table, given.tableStride,
-                         target, bias, scale, loss, lse);
+    // a block per row where a wave would walk more than four rounds of parts
+    const bool whole = plan.forward.parts >= 4 * kWave;
+    const dim3 grid((unsigned)std::min(whole ? rows : cdiv(rows, kBlock / kWave), kMostBlocks));
+    if (whole) {
+        RECSDK_LAUNCH_AS("k_softmax_loss_join", (k_softmax_loss_join<T, kBlock>), grid, dim3(kBlock), stream, a.norm,
+                         plan.forward.parts, (int)rows, (int)items, dim, x, given.xStride, table, given.tableStride, target, bias,
+                         scale, loss, lse);
     } else {
-        RECSDK_LAUNCH_AS("k_softmax_loss_join", (k_softmax_loss_join<T, kWave>), dim3((unsigned)cdiv(rows, kBlock / kWave)),
-                         dim3(kBlock), stream, a.norm, plan.forward.parts, (int)rows, (int)items, dim, x, given.xStride, table,
-                         given.tableStride, target, bias, scale, loss, lse);
+        RECSDK_LAUNCH_AS("k_softmax_loss_join", (k_softmax_loss_join<T, kWave>), grid, dim3(kBlock), stream, a.norm,
+                         plan.forward.parts, (int)rows, (int)items, dim, x, given.xStride, table, given.tableStride, target, bias,
+                         scale, loss, lse);
     }
     return RECSDK_OK;
 }

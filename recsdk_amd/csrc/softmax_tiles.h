@@ -101,8 +101,10 @@ constexpr int narrow_waves(int planes, int dp) { return planes == 3 && dp > 128 
 // memory and LDS, would be too many.
 constexpr int tile_rows(int planes, int dp, int ownWaves, int pass)
 {
-    return ownWaves < 4                                                                            ? 32 * (4 / ownWaves)
-           : planes == 1 ? (dp > 160 && pass != kLossForward ? 32 : 64) : planes == 2 ? (dp > 64 ? 32 : 64) : dp > 32 ? 32 : 64;
+    if (ownWaves < 4) {
+        return 32 * (4 / ownWaves);
+    }
+    return planes == 1 ? (dp > 160 && pass != kLossForward ? 32 : 64) : planes == 2 ? (dp > 64 ? 32 : 64) : dp > 32 ? 32 : 64;
 }
 
 // Waves per SIMD that the registers have to leave room for.
@@ -277,7 +279,8 @@ template <int P, int DP, int RW, int OW, int PASS>
 struct LossTile {
     static constexpr int kColBlocks = RW / 32;
     static constexpr int kSteps = DP / 16;
-    static constexpr int kRowThreads = DP <= 32 ? 4 : DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // threads that move a row, 8 columns each
+    // threads that move a row, 8 columns each
+    static constexpr int kRowThreads = DP <= 32 ? 4 : DP <= 64 ? 8 : DP <= 128 ? 16 : 32;
     static constexpr int kStreamWaves = 4 / OW;
     static constexpr int kRows = tile_rows(P, DP, OW, PASS);
     static constexpr int kLoads = kRows * kRowThreads / kLossThreads;   // chunks per thread and tile
@@ -288,7 +291,6 @@ struct LossTile {
     static_assert(P * kPlane * 2 * kBuffers <= 147456, "the tiles fit LDS");
 };
 
-//
 // SHIFT: scores are shifted by a value per item (item_bias, or minus infinity past the end of the table).  A kernel without
 // it takes the last, partial tile with it in a loop of its own: one loop with both forms in it made the compiler move the
 // accumulators from registers to registers in every round.
@@ -471,7 +473,8 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                 }
             }
             if (threadIdx.x < TR) {
-                auxA[buf][(threadIdx.x & ~31) | tile_row(threadIdx.x & 31)] = t * TR + (int)threadIdx.x < a.streams ? 0.0f : -INFINITY;
+                const int at = (threadIdx.x & ~31) | tile_row(threadIdx.x & 31);
+                auxA[buf][at] = t * TR + (int)threadIdx.x < a.streams ? 0.0f : -INFINITY;
             }
         }
 #pragma unroll
@@ -674,7 +677,8 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                     float high = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        s[cb][i] = __builtin_fmaf(s[cb][i], c2, shifted || P == 2 ? shift[i] + (ownShift[cb] + lift[cb]) : shift[i]);
+                        s[cb][i] = __builtin_fmaf(s[cb][i], c2,
+                                                  shifted || P == 2 ? shift[i] + (ownShift[cb] + lift[cb]) : shift[i]);
                         high = fmaxf(high, s[cb][i]);
                     }
                     if constexpr (P == 2) {
@@ -733,7 +737,8 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
             // piece holds a target, whose value is nearly the whole gradient of its row, a second round adds what the rounding
             // of the values has left, so that most gradients are off by their own rounding alone.  (A loop, not a branch with
             // the product in it a second time: that made the compiler keep the accumulators twice.)
-            const E* columnAt = &tile[buf][(r0 + 4 * ((lane & 15) >> 2) + half) * L::kRow + ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
+            const int rowOf = r0 + 4 * ((lane & 15) >> 2) + half;
+            const E* columnAt = &tile[buf][rowOf * L::kRow + ((lane >> 4) & 1) * 16 + (lane & 3) * 4];
             bool again = P == 1 && hit;
 #pragma unroll 1
             while (true) {

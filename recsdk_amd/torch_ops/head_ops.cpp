@@ -241,9 +241,7 @@ public:
     {
         auto [y, mean, rstd] = norm_forward(x, weight, bias, eps, true, "recsdk::layer_norm");
         ctx->save_for_backward({x, mean, rstd, has(weight) ? *weight : Tensor()});
-        ctx->saved_data["dweight"] = has(weight) && weight->requires_grad();
-        ctx->saved_data["dbias"] = has(bias) && bias->requires_grad();
-        ctx->saved_data["dx"] = x.requires_grad();
+        ctx->saved_data["biased"] = has(bias);
         ctx->saved_data["bias_type"] = has(bias) ? (int64_t)bias->scalar_type() : (int64_t)at::kFloat;
         return y;
     }
@@ -257,9 +255,11 @@ public:
         }
         const auto saved = ctx->get_saved_variables();
         const optional<Tensor> weight = saved[3].defined() ? optional<Tensor>(saved[3]) : optional<Tensor>();
-        auto [dx, dw, db] = layer_norm_backward(
-            grads[0], saved[0], weight, saved[1], saved[2],
-            {ctx->saved_data["dx"].toBool(), ctx->saved_data["dweight"].toBool(), ctx->saved_data["dbias"].toBool()});
+        // the inputs that are tensors are counted: the bias is the second of them without a weight
+        const bool weighted = weight.has_value();
+        const std::array<bool, 3> wanted = {ctx->needs_input_grad(0), weighted && ctx->needs_input_grad(1),
+                                            ctx->saved_data["biased"].toBool() && ctx->needs_input_grad(weighted ? 2 : 1)};
+        auto [dx, dw, db] = layer_norm_backward(grads[0], saved[0], weight, saved[1], saved[2], wanted);
         out[0] = dx;
         out[1] = dw;
         if (db.defined()) {
@@ -396,8 +396,6 @@ public:
         auto [loss, lse] = softmax_loss_forward(x, table, target, item_bias, scale);
         ctx->save_for_backward({x, table, target, lse, has(item_bias) ? *item_bias : Tensor()});
         ctx->saved_data["scale"] = scale;
-        ctx->saved_data["dx"] = x.requires_grad();
-        ctx->saved_data["dtable"] = table.requires_grad();
         return loss;
     }
 
@@ -412,7 +410,7 @@ public:
         const optional<Tensor> bias = saved[4].defined() ? optional<Tensor>(saved[4]) : optional<Tensor>();
         std::tie(out[0], out[1]) =
             softmax_loss_backward(grads[0], saved[0], saved[1], saved[2], saved[3], bias, ctx->saved_data["scale"].toDouble(),
-                                  {ctx->saved_data["dx"].toBool(), ctx->saved_data["dtable"].toBool()});
+                                  {ctx->needs_input_grad(0), ctx->needs_input_grad(1)});
         return out;
     }
 };

@@ -614,6 +614,70 @@ def test_bfloat16_gradients_are_off_by_their_own_rounding(ops, each):
         assert (a.double() - exact).norm() <= 1.15 * own
 
 
+# ---- more rows than one launch has blocks for, rows far apart, gradients asked for one by one ---------------------------------
+
+def test_layer_norm_more_wide_rows_than_blocks(ops):
+    # rows off the 16-byte borders, with gaps, past what a block holds: a block per row, for 65536 of them at a time
+    rows, dim = 65600, 4097
+    wide = torch.randn(rows, dim + 2, generator=torch.Generator(DEV).manual_seed(90), device=DEV).bfloat16()
+    x = wide[:, 1:dim + 1]
+    weight = 1 + randn(dim, seed=91, std=0.1)
+    bias = randn(dim, seed=92)
+    grad = torch.zeros(rows, dim, dtype=torch.bfloat16, device=DEV)
+    grad[-100:] = randn(100, dim, seed=93, dtype=torch.bfloat16)
+    y, mean, rstd = ops.layer_norm_forward(x, weight, bias)
+    dx, dw, db = ops.layer_norm_backward(grad, x, weight, mean, rstd, [True, True, True])
+    some = torch.cat([torch.arange(40), torch.arange(rows - 100, rows)]).to(DEV)
+    want = plain.layer_norm(x[some], weight, bias, 1e-5, grad[some])
+    plain.close(y[some], want[0], "y")
+    plain.close(dx[some], want[1], "dx")
+    plain.close(dw, want[2], "dweight")   # the other rows' gradients are zero
+    plain.close(db, want[3], "dbias")
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_softmax_loss_more_rows_than_blocks(ops, kind):
+    x, table, target, grad = loss_case(525_000, 9, 5, kind, 94)   # padded rows, 65536 blocks of eight of them at a time
+    check_loss(ops, x, table, target, None, 0.5, grad)
+
+
+def test_softmax_loss_large_table_and_no_rows(ops):
+    x, table, target, grad = loss_case(4, 300_000, 256, "bf16", 95)
+    torch.full_like(table, 7.0)   # what the gradient's memory may hold before
+    _, dt = ops.softmax_loss_backward(grad[:0], x[:0], table, target[:0], grad[:0], None, 1.0, [False, True])
+    assert not dt.any()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_softmax_loss_rows_far_apart(ops, kind):
+    x, table, target, grad = loss_case(5, 9, 64, kind, 96)
+    far = torch.zeros(9, 2 ** 22 + 8, dtype=TYPES[kind], device=DEV)
+    far[:, :64] = table
+    check_loss(ops, x, far[:, :64], target, None, 0.4, grad)
+    far[:5, :64] = x
+    check_loss(ops, far[:5, :64], table, target, None, 0.4, grad)
+
+
+@pytest.mark.parametrize("weighted", [True, False])
+def test_gradients_of_some_inputs_only(ops, weighted):
+    x, weight, bias, grad = norm_case(70, 100, "f32", "f32", 97)
+    leaves = [t.requires_grad_() for t in ((x, weight, bias) if weighted else (x, bias))]
+
+    def layer(inputs):
+        return ops.layer_norm(inputs[0], inputs[1] if weighted else None, inputs[-1])
+
+    whole = torch.autograd.grad(layer(leaves), leaves, grad)
+    for leaf, want in zip(leaves, whole):
+        assert torch.equal(torch.autograd.grad(layer(leaves), (leaf,), grad)[0], want)
+        only = [t if t is leaf else t.detach() for t in leaves]
+        assert torch.equal(torch.autograd.grad(layer(only), (leaf,), grad)[0], want)
+    x, table, target, grad = loss_case(70, 300, 64, "bf16", 98)
+    leaves = [x.requires_grad_(), table.requires_grad_()]
+    whole = torch.autograd.grad(ops.softmax_loss(*leaves, target), leaves, grad)
+    for leaf, want in zip(leaves, whole):
+        assert torch.equal(torch.autograd.grad(ops.softmax_loss(*leaves, target), (leaf,), grad)[0], want)
+
+
 # ---- refusals that need a device -------------------------------------------------------------------------------------
 
 def test_refusals_of_the_torch_operators(ops):

@@ -107,6 +107,21 @@ def test_softmax_loss_workspace_grows_with_what_is_copied():
     assert L.recsdk_softmax_loss_workspace(0, 1000, 64, BF16, 64, 64, f, b) == capi.OK and f.value == b.value == 0
 
 
+def test_softmax_loss_rows_far_apart_are_copied():
+    L, f, b = capi.lib(), ctypes.c_int64(), ctypes.c_int64()
+    assert L.recsdk_softmax_loss_workspace(100, 1000, 64, F32, 64, 2 ** 22, f, b) == capi.OK
+    near = f.value, b.value
+    assert L.recsdk_softmax_loss_workspace(100, 1000, 64, F32, 64, 2 ** 22 + 4, f, b) == capi.OK
+    assert f.value >= near[0] + 1000 * 64 * 4 and b.value >= near[1] + 1000 * 64 * 4
+
+
+def test_layer_norm_rows_too_long():
+    n = ctypes.c_int64()
+    assert capi.lib().recsdk_layer_norm_workspace(4, 2 ** 30, n) == capi.EINVAL
+    args = (SOME, 1, 2 ** 30, 2 ** 30, F32, None, None, F32, 1e-5, SOME, None, None, None)
+    assert capi.lib().recsdk_layer_norm_forward(*args) == capi.EINVAL and "dim" in text()
+
+
 def test_host_tensors_are_refused():
     torch_ops.load()
     ops = torch.ops.recsdk
