@@ -129,20 +129,31 @@ __global__ __launch_bounds__(kBlock) void k_softmax_grad_join(const float* __res
 }
 
 // Rows of `dim` elements at any stride -> rows of `padded` elements (whole 16-byte pieces), the rest zero.  32 threads take
-// a row's pieces.
+// a row's pieces; the first blocks take x's rows, the others the table's, in one launch (301 x 30011 x 201: 5 us less).
 template <typename T>
-__global__ __launch_bounds__(kBlock) void k_pad_rows(const T* __restrict__ src, int64_t stride, int64_t rows, int dim, int padded,
-                                                     T* __restrict__ dst)
+struct PadRows {
+    const T* src;
+    int64_t stride;
+    int64_t rows;
+    T* dst;
+    int64_t blocks;   // 0: as they are
+};
+
+template <typename T>
+__global__ __launch_bounds__(kBlock) void k_pad_rows(PadRows<T> x, PadRows<T> table, int dim, int padded)
 {
     constexpr int kPer = 16 / sizeof(T);
-    for (int64_t r = (int64_t)blockIdx.x * (kBlock / 32) + threadIdx.x / 32; r < rows; r += (int64_t)gridDim.x * (kBlock / 32)) {
+    const bool second = blockIdx.x >= x.blocks;
+    const PadRows<T> p = second ? table : x;
+    const int64_t first = blockIdx.x - (second ? x.blocks : 0);
+    for (int64_t r = first * (kBlock / 32) + threadIdx.x / 32; r < p.rows; r += p.blocks * (kBlock / 32)) {
         for (int c = threadIdx.x % 32 * kPer; c < padded; c += 32 * kPer) {
             Pack<T, kPer> v;
 #pragma unroll
             for (int e = 0; e < kPer; ++e) {
-                v.v[e] = c + e < dim ? src[r * stride + c + e] : from_float<T>(0.0f);
+                v.v[e] = c + e < dim ? p.src[r * p.stride + c + e] : from_float<T>(0.0f);
             }
-            *reinterpret_cast<Pack<T, kPer>*>(dst + r * padded + c) = v;
+            *reinterpret_cast<Pack<T, kPer>*>(p.dst + r * padded + c) = v;
         }
     }
 }
@@ -301,18 +312,6 @@ static int check_loss(const char* name, int64_t rows, int64_t items, int32_t dim
     return RECSDK_OK;
 }
 
-// The operands as the tile kernels read them: whole 16-byte pieces; others are copied into padded rows.
-template <typename T>
-static int pad_operand(const void*& p, int64_t& stride, int64_t rows, int dim, int padded, void* to, hipStream_t stream)
-{
-    const int64_t grid = std::min(cdiv(rows, kBlock / 32), kMostBlocks);
-    RECSDK_LAUNCH_AS("k_pad_rows", (k_pad_rows<T>), dim3((unsigned)grid), dim3(kBlock), stream, static_cast<const T*>(p), stride,
-                     rows, dim, padded, static_cast<T*>(to));
-    p = to;
-    stride = padded;
-    return RECSDK_OK;
-}
-
 template <typename T, int WAYS>
 static int launch_grad_join(const float* part, int parts, int64_t rows, int dim, const float* lse, const float* grad,
                             float scale, void* out, hipStream_t stream)
@@ -340,18 +339,26 @@ struct LossOperands {
     int64_t tableStride;
 };
 
+// The operands as the tile kernels read them: whole 16-byte pieces; others are copied into padded rows.
 template <typename T>
 static int pad_operands(const LossPlan& plan, LossOperands& o, int64_t rows, int64_t items, int dim, char* workspace,
                         hipStream_t stream)
 {
-    if (plan.padX) {
-        const int rc = pad_operand<T>(o.x, o.xStride, rows, dim, plan.padded, workspace + plan.atX, stream);
-        if (rc != RECSDK_OK) {
-            return rc;
+    auto padding = [&](bool wanted, const void*& src, int64_t& stride, int64_t count, int64_t at) {
+        PadRows<T> p{};
+        if (wanted) {
+            p = {static_cast<const T*>(src), stride, count, reinterpret_cast<T*>(workspace + at),
+                 std::min(cdiv(count, kBlock / 32), kMostBlocks)};
+            src = p.dst;
+            stride = plan.padded;
         }
-    }
-    if (plan.padTable) {
-        return pad_operand<T>(o.table, o.tableStride, items, dim, plan.padded, workspace + plan.atTable, stream);
+        return p;
+    };
+    const PadRows<T> x = padding(plan.padX, o.x, o.xStride, rows, plan.atX);
+    const PadRows<T> table = padding(plan.padTable, o.table, o.tableStride, items, plan.atTable);
+    if (x.blocks + table.blocks > 0) {
+        RECSDK_LAUNCH_AS("k_pad_rows", (k_pad_rows<T>), dim3((unsigned)(x.blocks + table.blocks)), dim3(kBlock), stream, x, table,
+                         dim, plan.padded);
     }
     return RECSDK_OK;
 }
