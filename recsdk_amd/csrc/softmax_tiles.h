@@ -70,12 +70,13 @@ struct LossArgs {
     const float* lse;       // backward: [rows of x], +inf where a row takes no gradient
     const float* grad;      // backward: [rows of x]
     float scale;
-    int32_t splits;         // pieces of the stream
+    int32_t whole;          // blocks of owners, the first ones, that take the whole stream (dt: and write their result)
+    int32_t splits;         // pieces of the stream for the others
     int32_t tilesPerSplit;
     float2* norm;           // forward: [split parts][owners] (maximum, sum), base 2
-    float* part;            // backward: [split parts][owners][partDim] partial sums, or NULL
+    float* part;            // backward: [split parts][owners past the whole blocks][partDim] partial sums
     int32_t partDim;        // dim rounded up to whole fours
-    void* out;              // dt pass without parts: [owners][dim] in the operands' type
+    void* out;              // dt: [owners][dim] in the operands' type, by the whole blocks
     const float* ownMax;    // P = 2: [kAbsMaxParts] largest values of the operands' rows
     const float* streamMax;
 };
@@ -137,6 +138,7 @@ struct PassPlan {
     int rowsPerWave;
     int ownWaves;
     int64_t blocks;
+    int64_t whole;   // the first of them take the whole stream; the others are cut into `splits`
     int splits;
     int tilesPerSplit;
     int parts;   // splits times the waves that share a block's stream
@@ -319,13 +321,14 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
     const int lane = lane_id();
     const int col = lane & 31;
     const int half = lane >> 5;
-    const int split = (int)(blockIdx.x % (unsigned)a.splits);
-    const int ownBlock = (int)(blockIdx.x / (unsigned)a.splits);
+    const bool cut = (int)blockIdx.x >= a.whole;
+    const int split = cut ? (int)((blockIdx.x - a.whole) % (unsigned)a.splits) : 0;
+    const int ownBlock = cut ? a.whole + (int)((blockIdx.x - a.whole) / (unsigned)a.splits) : (int)blockIdx.x;
     const int ownBase = (ownBlock * OW + wave % OW) * RW;
     const int streamWave = wave / OW;
     const int tiles = (a.streams + TR - 1) / TR;
     const int t0 = split * a.tilesPerSplit;
-    const int t1 = min(t0 + a.tilesPerSplit, tiles);   // t0 < t1: no split is empty
+    const int t1 = cut ? min(t0 + a.tilesPerSplit, tiles) : tiles;   // t0 < t1: no split is empty
     const bool biased = a.bias != nullptr;
     constexpr int kElement = P == 1 ? 2 : 4;
     float ownMost = 0.0f;
@@ -829,7 +832,8 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
         return;
     }
 
-    const int64_t partRow = (int64_t)(split * L::kStreamWaves + streamWave) * a.owners;
+    const int cutBase = a.whole * (OW * RW);   // the first owner of a cut block
+    const int64_t partRow = (int64_t)(split * L::kStreamWaves + streamWave) * (a.owners - cutBase) - cutBase;
     if constexpr (PASS == kLossForward) {
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
@@ -860,7 +864,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                 if (P == 2) {
                     v *= down;
                 }
-                if (a.part != nullptr) {
+                if (cut) {
                     store_columns(a.part + (partRow + n) * a.partDim, d, a.partDim, true, v);
                 } else if constexpr (P == 1) {
                     store_columns(static_cast<BF16*>(a.out) + (int64_t)n * a.dim, d, a.dim, fours, v);
@@ -876,7 +880,7 @@ template <int P, int DP, int RW, int OW, int PASS, bool SHIFT>
 int launch_tiles(const LossArgs& a, const PassPlan& p, hipStream_t stream)
 {
     const char* name = PASS == kLossForward ? "k_softmax_forward" : PASS == kLossDx ? "k_softmax_dx" : "k_softmax_dt";
-    RECSDK_LAUNCH_AS(name, (k_softmax_tiles<P, DP, RW, OW, PASS, SHIFT>), dim3((unsigned)(p.blocks * p.splits)),
+    RECSDK_LAUNCH_AS(name, (k_softmax_tiles<P, DP, RW, OW, PASS, SHIFT>), dim3((unsigned)(p.whole + (p.blocks - p.whole) * p.splits)),
                      dim3(kLossThreads), stream, a);
     return RECSDK_OK;
 }

@@ -641,6 +641,15 @@ def test_softmax_loss_more_rows_than_blocks(ops, kind):
     check_loss(ops, x, table, target, None, 0.5, grad)
 
 
+@pytest.mark.parametrize("kind,rows,items,dim", [("f32", 801, 33001, 200), ("bf16", 642, 65800, 250)])
+def test_softmax_loss_last_items_in_pieces(ops, kind, rows, items, dim):
+    # one round of blocks over the items and a few more blocks, which share out the rows of x
+    x, table, target, grad = loss_case(rows, items, dim, kind, 99)
+    target[::7] = torch.randint(items - 300, items, (target[::7].numel(),), generator=torch.Generator().manual_seed(100)).to(DEV)
+    target[3] = -1
+    check_loss(ops, x, table, target, None, 3 / math.sqrt(dim), grad)
+
+
 def test_softmax_loss_large_table_and_no_rows(ops):
     x, table, target, grad = loss_case(4, 300_000, 256, "bf16", 95)
     torch.full_like(table, 7.0)   # what the gradient's memory may hold before
