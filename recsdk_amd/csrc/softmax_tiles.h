@@ -95,8 +95,8 @@ constexpr int loss_width(int dim) { return (dim + 31) / 32 * 32; }
 constexpr int wide_rows(int planes, int dp, int pass) { return planes == 1 && (dp <= 96 || pass == kLossForward) ? 64 : 32; }
 
 // Waves that own rows of their own where there are at most 32 rows: all would own padding but one, so they share the stream
-// instead (all four, unless their tile is too large for LDS).
-constexpr int narrow_waves(int planes, int dp) { return planes == 3 && dp > 128 ? 2 : 1; }
+// instead (all four, unless two such tiles do not fit LDS).
+constexpr int narrow_waves(int planes, int dp) { return planes == 3 && dp > 64 ? 2 : 1; }
 
 // Rows of a tile: 32 for each wave that shares the stream; else 64, or 32 where two buffers of LDS, or the registers between
 // memory and LDS, would be too many.
@@ -108,11 +108,18 @@ constexpr int tile_rows(int planes, int dp, int ownWaves, int pass)
     return planes == 1 ? (dp > 160 && pass != kLossForward ? 32 : 64) : planes == 2 ? (dp > 64 ? 32 : 64) : dp > 32 ? 32 : 64;
 }
 
+// Few rows: one buffer of LDS where a compute unit then holds two blocks, with twice the loads in flight (1 x 1 M x 64 float32,
+// forward: 79 us with two buffers, 56 with one; 8 x 400000 x 160 bfloat16: 35 and 28).
+constexpr bool single_buffer(int planes, int dp, int ownWaves, int pass)
+{
+    return ownWaves < 4 && (planes == 3 || (dp > 128 && (pass == kLossForward || dp <= 160)));
+}
+
 // Waves per SIMD that the registers have to leave room for.
 constexpr int loss_waves(int planes, int dp, int ownWaves, int pass)
 {
     if (ownWaves < 4) {
-        return dp >= 128 || (planes == 3 && dp >= 64) ? 1 : 2;
+        return planes == 3 ? (dp > 128 ? 1 : 2) : pass == kLossForward || dp <= 160 ? 2 : 1;
     }
     if (pass == kLossForward) {
         return planes == 1 && dp > 224 ? 1 : 2;
@@ -126,7 +133,7 @@ constexpr int resident_blocks(int planes, int dp, int pass)
     if (pass == kLossForward) {
         return planes == 1   ? (dp <= 64 ? 4 : dp <= 128 ? 3 : dp <= 224 ? 2 : 1)
                : planes == 2 ? (dp <= 64 ? 4 : dp <= 128 ? 3 : 2)
-                             : (dp <= 32 ? 4 : dp <= 64 ? 3 : dp <= 128 ? 2 : 1);
+                             : (dp <= 32 ? 4 : dp <= 128 ? 2 : 1);
     }
     return planes == 1   ? (dp <= 32 ? 3 : 2)
            : planes == 2 ? (dp <= 32 ? 4 : dp <= 64 ? 3 : dp <= 160 ? 2 : 1)
@@ -288,7 +295,7 @@ struct LossTile {
     static constexpr int kLoads = kRows * kRowThreads / kLossThreads;   // chunks per thread and tile
     static constexpr int kRow = DP + 8;                                 // elements from row to row
     static constexpr int kPlane = kRows * kRow;
-    static constexpr int kBuffers = P * kPlane * 2 * 2 > 147456 ? 1 : 2;
+    static constexpr int kBuffers = P * kPlane * 2 * 2 > 147456 || single_buffer(P, DP, OW, PASS) ? 1 : 2;
     static_assert(kLoads >= 1 && kLoads * kLossThreads == kRows * kRowThreads, "whole chunks per thread");
     static_assert(P * kPlane * 2 * kBuffers <= 147456, "the tiles fit LDS");
 };
