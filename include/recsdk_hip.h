@@ -767,13 +767,14 @@ RECSDK_API int recsdk_layer_norm_backward(const void* d_grad, const void* d_x, i
  *                  item out: a free slot of the table, whose row may hold anything.  A row whose target is taken out
  *                  (so also one that no item is left for) has loss +infinity and gives no gradient
  *   d_loss, d_lse  [rows] fp32; d_lse is for the backward pass: log-sum-exp, or +infinity where a row gives no gradient
- *   scale          any finite value
+ *   scale          finite; for bf16 rows with d_item_bias 0, or at least 2^-40 in size
  * d_x, d_table, d_workspace, and the gradients d_dx and d_dtable are 16-byte aligned.  rows and items < 2^30, items >= 1.
  * Rows that are no whole 16-byte pieces, or more than 2^22 elements apart, are copied into the workspace first.
  * Sums and statistics are fp32.  The gradients take (probability - [target]) grad in the operands' precision: bf16 in one
  * rounding, and a second one of what the first has left where a target is among 32 rows at a time.  fp32 products of more
  * than 32 rows keep 22 bits of each value, and of an operand nothing below 2^-40 of its largest finite one, in rows and items that
- * take part; an infinity in one of those rows or items counts as NaN.  Products of up to 32 rows keep 24 bits. */
+ * take part (of dtable's (probability - [target]) grad, 2^-32 of the item's largest); an infinity in one of those rows or items
+ * counts as NaN.  Products of up to 32 rows keep 24 bits. */
 RECSDK_API int recsdk_softmax_loss_workspace(int64_t rows, int64_t items, int32_t dim, int32_t dtype, int64_t x_stride,
                                              int64_t table_stride, int64_t* h_forward_bytes, int64_t* h_backward_bytes);
 RECSDK_API int recsdk_softmax_loss_forward(const void* d_x, int64_t rows, int64_t x_stride, const void* d_table, int64_t items,

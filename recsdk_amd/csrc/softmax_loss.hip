@@ -361,6 +361,17 @@ struct LossOperands {
     int64_t tableStride;
 };
 
+// item_bias / scale is what the bfloat16 kernels work with (folds_shift)
+static int check_scale(const char* name, int32_t dtype, const float* bias, float scale)
+{
+    const float size = scale < 0.0f ? -scale : scale;
+    if (!(size < INFINITY) || (dtype == RECSDK_DT_BF16 && bias != nullptr && size != 0.0f && size < 0x1p-40f)) {
+        set_error("%s: scale must be finite, and 0 or at least 2^-40 for bf16 rows with item_bias", name);
+        return RECSDK_EINVAL;
+    }
+    return RECSDK_OK;
+}
+
 // The operands as the tile kernels read them: whole 16-byte pieces; others are copied into padded rows.
 template <typename T>
 static int pad_operands(const LossPlan& plan, LossOperands& o, int64_t rows, int64_t items, int dim, char* workspace,
@@ -540,7 +551,8 @@ extern "C" int recsdk_softmax_loss_forward(const void* d_x, int64_t rows, int64_
                                            int64_t workspace_bytes, void* stream)
 {
     using namespace recsdk;
-    const int rc = check_loss("recsdk_softmax_loss_forward", rows, items, dim, dtype, x_stride, table_stride);
+    int rc = check_loss("recsdk_softmax_loss_forward", rows, items, dim, dtype, x_stride, table_stride);
+    rc = rc == RECSDK_OK ? check_scale("recsdk_softmax_loss_forward", dtype, d_item_bias, scale) : rc;
     if (rc != RECSDK_OK) {
         return rc;
     }
@@ -568,7 +580,8 @@ extern "C" int recsdk_softmax_loss_backward(const float* d_grad_loss, const void
                                             void* d_dx, void* d_dtable, void* d_workspace, int64_t workspace_bytes, void* stream)
 {
     using namespace recsdk;
-    const int rc = check_loss("recsdk_softmax_loss_backward", rows, items, dim, dtype, x_stride, table_stride);
+    int rc = check_loss("recsdk_softmax_loss_backward", rows, items, dim, dtype, x_stride, table_stride);
+    rc = rc == RECSDK_OK ? check_scale("recsdk_softmax_loss_backward", dtype, d_item_bias, scale) : rc;
     if (rc != RECSDK_OK) {
         return rc;
     }

@@ -140,6 +140,17 @@ constexpr int resident_blocks(int planes, int dp, int pass)
                          : (dp <= 32 ? 4 : dp <= 128 ? 2 : 1);
 }
 
+// Whether a stream row's shift of the scores goes into the first product's accumulators, read from LDS, instead of being added
+// to each score afterwards.  bfloat16 with item_bias, forward, 8192 x 200003 x 64: 433 us added, 398 folded (4096 x 50000 x 256:
+// 144 and 156).  The backward passes wait for those reads about as long as for the addition (4096 x 50000 x 192, dt: 221 and
+// 226; 128 columns: 158 and 168), but where they are short of registers it holds 16 fewer (dt, 96 columns: 256 and 231;
+// 224: 296 and 240; 256: 457 and 382; dx, 256: 280 and 233).  float32 adds: its products are scaled by the operands' largest
+// values, where a shift might not fit.
+constexpr bool folds_shift(int planes, int dp, int pass)
+{
+    return planes == 1 && (pass == kLossForward ? dp <= 224 : pass == kLossDx ? dp > 224 : dp == 96 || dp > 128);
+}
+
 // What one pass launches.
 struct PassPlan {
     int rowsPerWave;
@@ -337,6 +348,15 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
     const int t0 = split * a.tilesPerSplit;
     const int t1 = cut ? min(t0 + a.tilesPerSplit, tiles) : tiles;   // t0 < t1: no split is empty
     const bool biased = a.bias != nullptr;
+    // the forward pass bounds scores by the largest product, so there a negative scale goes into the owner's rows
+    const bool turned = PASS == kLossForward && a.scale < 0.0f;
+    // a shift is divided by the scale and goes into the product as what that adds to; without a scale, rows of zeros take its
+    // place
+    constexpr bool kFold = folds_shift(P, DP, PASS);
+    const bool still = kFold && a.scale == 0.0f;
+    float c2 = (still ? 1.0f : turned ? -a.scale : a.scale) * kLog2e;
+    const float fold = kFold ? 1.0f / c2 : 1.0f;
+    const float gone = kFold && c2 < 0.0f ? INFINITY : -INFINITY;   // the shift of a row that takes no part
     constexpr int kElement = P == 1 ? 2 : 4;
     float ownMost = 0.0f;
     float streamMost = 0.0f;
@@ -436,10 +456,13 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                 x.minus = g < 0.0f;
                 x.g = fabsf(g);
                 x.a = x.dead ? -INFINITY : log2f(x.g) - x.a * kLog2e;
+                if constexpr (SHIFT) {
+                    x.a = kFold ? x.a * fold : x.a;
+                }
                 x.t = x.dead ? -1 : x.t;
             } else {
                 x.dead = x.dead || x.a <= kMaskedBelow;
-                x.a = x.dead ? -INFINITY : x.a * kLog2e;
+                x.a = x.dead ? gone : x.a * (kLog2e * fold);
             }
             const unsigned long long dead = __ballot(x.dead);
             if (threadIdx.x < TR && (lane & 31) == 0) {
@@ -484,7 +507,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
             }
             if (threadIdx.x < TR) {
                 const int at = (threadIdx.x & ~31) | tile_row(threadIdx.x & 31);
-                auxA[buf][at] = t * TR + (int)threadIdx.x < a.streams ? 0.0f : -INFINITY;
+                auxA[buf][at] = t * TR + (int)threadIdx.x < a.streams ? 0.0f : gone;
             }
         }
 #pragma unroll
@@ -505,9 +528,6 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
     Aux next = aux_load(t0);   // of the tile that is placed next
     Aux second = aux_load(t0 + 1);
     fetch(t0);
-    // the forward pass bounds scores by the largest product, so there a negative scale goes into the owner's rows
-    const bool turned = PASS == kLossForward && a.scale < 0.0f;
-    float c2 = (turned ? -a.scale : a.scale) * kLog2e;
     if constexpr (P == 2) {
         float* largest = &auxA[0][0];   // free until the first tile is placed
         const float o = wave_max(ownMost);
@@ -537,7 +557,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            if (!live) {
+            if (!live || still) {
                 ownRaw[cb][ks].clear();   // rows past the end, padding positions and free slots may hold anything
             }
             if (turned) {
@@ -571,12 +591,29 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
     auto piece = [&](auto shiftedC, int buf, int r0, int rowBase) {
         constexpr bool shifted = decltype(shiftedC)::value;
         const E* rowAt = &tile[buf][(r0 + tile_row(col)) * L::kRow + half * 8];
+        constexpr bool folded = shifted && kFold;
+        auto shifts = [&](float (&b)[16], int row0) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const Float4 v = *reinterpret_cast<const Float4*>(&auxA[buf][row0 + 8 * q + 4 * half]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    b[4 * q + j] = v[j];
+                }
+            }
+        };
         Float16 s[CB];
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
+            float b[16];
+            if constexpr (folded) {
+                int row0 = r0;
+                pin(row0);   // loads of its own for each: copies would take an instruction per score
+                shifts(b, row0);
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                s[cb][i] = 0.0f;
+                s[cb][i] = folded ? b[i] : 0.0f;
             }
         }
 #pragma unroll
@@ -595,15 +632,9 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
         if constexpr (PASS == kLossForward) {
             float b[16];
             float most = 0.0f;   // largest shift
-            if constexpr (shifted) {
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const Float4 v = *reinterpret_cast<const Float4*>(&auxA[buf][r0 + 8 * q + 4 * half]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        b[4 * q + j] = v[j];
-                    }
-                }
+            constexpr bool add = shifted && !folded;
+            if constexpr (add) {
+                shifts(b, r0);
                 most = b[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) {
@@ -623,32 +654,26 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                     float now = top[cb];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        now = fmaxf(now, shifted ? __builtin_fmaf(s[cb][i], c2, b[i]) : s[cb][i] * c2);
+                        now = fmaxf(now, add ? __builtin_fmaf(s[cb][i], c2, b[i]) : s[cb][i] * c2);
                     }
                     sum[cb] *= exp2_fast(top[cb] - now);
                     top[cb] = now;
                 }
-                float add = 0.0f;
+                float more = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
-                    add += exp2_fast(__builtin_fmaf(s[cb][i], c2, shifted ? b[i] - top[cb] : -top[cb]));
+                    more += exp2_fast(__builtin_fmaf(s[cb][i], c2, add ? b[i] - top[cb] : -top[cb]));
                 }
-                sum[cb] += add;
+                sum[cb] += more;
             }
         } else {
             Frag<P> g[CB][2][P];
             bool hit = false;   // the piece holds a target of the wave's rows
             if constexpr (PASS == kLossDx) {
                 float b[16];
-                if constexpr (shifted) {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const Float4 v = *reinterpret_cast<const Float4*>(&auxA[buf][r0 + 8 * q + 4 * half]);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            b[4 * q + j] = v[j];
-                        }
-                    }
+                constexpr bool add = shifted && !folded;
+                if constexpr (add) {
+                    shifts(b, r0);
                 }
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
@@ -656,7 +681,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                     constexpr float kOne = P == 2 ? 32768.0f : 1.0f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        s[cb][i] = exp2_fast(__builtin_fmaf(s[cb][i], c2, shifted ? b[i] + shift : shift));
+                        s[cb][i] = exp2_fast(__builtin_fmaf(s[cb][i], c2, add ? b[i] + shift : shift));
                     }
                     int d = ownTarget[cb] - rowBase;
                     if (__any((unsigned)d < 32u)) {
@@ -672,13 +697,8 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
             } else {
                 // |grad scale| is in the exponent; its sign, and the 1 at the target, are rarely asked for
                 float shift[16];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const Float4 v = *reinterpret_cast<const Float4*>(&auxA[buf][r0 + 8 * q + 4 * half]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        shift[4 * q + j] = v[j];
-                    }
+                if constexpr (!folded) {
+                    shifts(shift, r0);
                 }
                 hit = __any((unsigned)(auxT[buf][r0 + col] - ownBase) < (unsigned)RW);
                 const uint32_t minus = __builtin_amdgcn_readfirstlane(minusBits[buf][r0 / 32]);
@@ -687,8 +707,12 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                     float high = -INFINITY;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        s[cb][i] = __builtin_fmaf(s[cb][i], c2,
-                                                  shifted || P == 2 ? shift[i] + (ownShift[cb] + lift[cb]) : shift[i]);
+                        if constexpr (folded) {
+                            s[cb][i] = __builtin_fmaf(s[cb][i], c2, ownShift[cb]);
+                        } else {
+                            s[cb][i] = __builtin_fmaf(s[cb][i], c2,
+                                                      shifted || P == 2 ? shift[i] + (ownShift[cb] + lift[cb]) : shift[i]);
+                        }
                         high = fmaxf(high, s[cb][i]);
                     }
                     if constexpr (P == 2) {
@@ -701,11 +725,13 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                                 high = fmaxf(high, auxT[buf][m] == mine ? log2f(auxG[buf][m]) + lift[cb] : -INFINITY);
                             }
                         }
-                        // Follows the item's largest value down, half of float16's reach at a time.  A half wave holds half of
-                        // the item's scores and of its columns' sums: both have to follow alike.
+                        // Follows the item's largest value down, half of float16's reach at a time (2 bits at a time cost 4 %
+                        // of the pass), but not below a target's, which is the largest but for another row's |grad|: what is
+                        // left out beside the largest is 2^-40 of a target's value, 2^-32 of others.  A half wave holds half
+                        // of the item's scores and of its columns' sums: both have to follow alike.
                         if (__any(high > kLift)) {
                             high = fmaxf(high, __shfl_xor(high, 32, kWave));
-                            const float down = high > kLift ? ceilf(high - kLift / 2) : 0.0f;
+                            const float down = high > kLift ? ceilf(high - (hit ? kLift : kLift / 2)) : 0.0f;
                             const float factor = exp2_fast(-down);
                             lift[cb] -= down;
 #pragma unroll
@@ -887,8 +913,8 @@ template <int P, int DP, int RW, int OW, int PASS, bool SHIFT>
 int launch_tiles(const LossArgs& a, const PassPlan& p, hipStream_t stream)
 {
     const char* name = PASS == kLossForward ? "k_softmax_forward" : PASS == kLossDx ? "k_softmax_dx" : "k_softmax_dt";
-    RECSDK_LAUNCH_AS(name, (k_softmax_tiles<P, DP, RW, OW, PASS, SHIFT>), dim3((unsigned)(p.whole + (p.blocks - p.whole) * p.splits)),
-                     dim3(kLossThreads), stream, a);
+    const int64_t grid = p.whole + (p.blocks - p.whole) * p.splits;
+    RECSDK_LAUNCH_AS(name, (k_softmax_tiles<P, DP, RW, OW, PASS, SHIFT>), dim3((unsigned)grid), dim3(kLossThreads), stream, a);
     return RECSDK_OK;
 }
 

@@ -327,6 +327,20 @@ def test_softmax_loss_large_negative_zero_and_sharp_scores(ops, kind):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [20, 64, 90, 128, 200, 224, 256])
+@pytest.mark.parametrize("rows", [6, 70, 300])
+def test_softmax_loss_scales_with_a_bias(ops, kind, dim, rows):
+    x, table, target, grad = loss_case(rows, 301, dim, kind, 20 + dim)
+    bias = 5 * torch.randn(301, generator=torch.Generator().manual_seed(dim)).to(DEV)
+    free = torch.arange(301, device=DEV) % 5 == 2
+    bias[free] = -math.inf
+    table[free] = math.nan
+    target = torch.where(free[target], target - 1, target)
+    for scale in (0.0, -0.3, 1e-6, 2.0 ** -40):
+        check_loss(ops, x, table, target, bias, scale, grad)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_softmax_loss_strided_rows(ops, kind):
     x, table, target, grad = loss_case(45, 400, 64, kind, 7)
     wide = randn(400, 192, seed=8, dtype=TYPES[kind])   # [row | state | state]: rows with optimizer state behind them

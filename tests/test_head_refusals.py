@@ -1,5 +1,6 @@
 """The training head's argument checks: everything here is refused on the host, before any HIP call."""
 import ctypes
+import math
 
 import pytest
 import torch
@@ -105,6 +106,15 @@ def test_softmax_loss_workspace_grows_with_what_is_copied():
     assert L.recsdk_softmax_loss_workspace(100, 1000, 64, BF16, 64, 65, f, b) == capi.OK   # table rows off the 16-byte border
     assert f.value >= plain[0] + 1000 * 64 * 2 and b.value >= plain[1] + 1000 * 64 * 2
     assert L.recsdk_softmax_loss_workspace(0, 1000, 64, BF16, 64, 64, f, b) == capi.OK and f.value == b.value == 0
+
+
+@pytest.mark.parametrize("dtype,bias,scale", [(F32, None, math.inf), (BF16, None, -math.inf), (F32, SOME, math.nan), (BF16, SOME, 1e-13),
+                                              (BF16, SOME, -1e-30)])
+def test_softmax_loss_scales(dtype, bias, scale):
+    L = capi.lib()
+    args = (SOME, 4, 8, SOME, 9, 8, 8, dtype, SOME, bias, scale)
+    assert L.recsdk_softmax_loss_forward(*args, SOME, SOME, SOME, 1 << 30, None) == capi.EINVAL and "scale" in text()
+    assert L.recsdk_softmax_loss_backward(SOME, *args, SOME, SOME, SOME, SOME, 1 << 30, None) == capi.EINVAL and "scale" in text()
 
 
 def test_softmax_loss_rows_far_apart_are_copied():
