@@ -171,6 +171,7 @@ int launch_f32_backward(int pass, int planes, const LossArgs& a, const PassPlan&
 #ifdef RECSDK_SOFTMAX_KERNELS
 
 typedef short Short4 __attribute__((ext_vector_type(4)));
+typedef int32_t Int4 __attribute__((ext_vector_type(4)));
 typedef float Float16 __attribute__((ext_vector_type(16)));
 
 // 16-bit elements of the planes
@@ -701,6 +702,15 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                     shifts(shift, r0);
                 }
                 hit = __any((unsigned)(auxT[buf][r0 + col] - ownBase) < (unsigned)RW);
+                // four rows' targets and |grad scale|, all loaded: a load of what a comparison asks for would wait for it
+                struct Hits {
+                    Int4 t;
+                    Float4 g;
+                };
+                auto hits = [&](int row) {
+                    return Hits{*reinterpret_cast<const Int4*>(&auxT[buf][r0 + row + 4 * half]),
+                                *reinterpret_cast<const Float4*>(&auxG[buf][r0 + row + 4 * half])};
+                };
                 const uint32_t minus = __builtin_amdgcn_readfirstlane(minusBits[buf][r0 / 32]);
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
@@ -719,11 +729,16 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                         if (hit) {   // the 1 at the target is the largest there is
                             int mine = ownBase + cb * 32 + col;
                             pin(mine);
+                            float largest = 0.0f;
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) {
-                                const int m = r0 + 8 * (i / 4) + 4 * half + i % 4;
-                                high = fmaxf(high, auxT[buf][m] == mine ? log2f(auxG[buf][m]) + lift[cb] : -INFINITY);
+                            for (int q = 0; q < 4; ++q) {
+                                const Hits h = hits(8 * q);
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) {
+                                    largest = fmaxf(largest, h.t[j] == mine ? h.g[j] : 0.0f);
+                                }
                             }
+                            high = fmaxf(high, log2f(largest) + lift[cb]);
                         }
                         // Follows the item's largest value down, half of float16's reach at a time (2 bits at a time cost 4 %
                         // of the pass), but not below a target's, which is the largest but for another row's |grad|: what is
@@ -756,9 +771,12 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                         pin(mine);
                         const float raise = P == 2 ? exp2_fast(lift[cb]) : 1.0f;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int m = r0 + 8 * (i / 4) + 4 * half + i % 4;
-                            s[cb][i] -= auxT[buf][m] == mine ? auxG[buf][m] * raise : 0.0f;
+                        for (int q = 0; q < 4; ++q) {
+                            const Hits h = hits(8 * q);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                s[cb][4 * q + j] -= h.t[j] == mine ? h.g[j] * raise : 0.0f;
+                            }
                         }
                     }
                     if (minus != 0) {
