@@ -588,29 +588,28 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
         }
     }
 
-    // ---- one 32-row piece of a tile ----
-    auto piece = [&](auto shiftedC, int buf, int r0, int rowBase) {
+    // ---- one 32-row piece of a tile: its scores, and what becomes of them ----
+    auto shifts = [&](float (&b)[16], int buf, int row0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const Float4 v = *reinterpret_cast<const Float4*>(&auxA[buf][row0 + 8 * q + 4 * half]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                b[4 * q + j] = v[j];
+            }
+        }
+    };
+    auto score = [&](auto shiftedC, Float16 (&s)[CB], int buf, int r0) {
         constexpr bool shifted = decltype(shiftedC)::value;
         const E* rowAt = &tile[buf][(r0 + tile_row(col)) * L::kRow + half * 8];
         constexpr bool folded = shifted && kFold;
-        auto shifts = [&](float (&b)[16], int row0) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const Float4 v = *reinterpret_cast<const Float4*>(&auxA[buf][row0 + 8 * q + 4 * half]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    b[4 * q + j] = v[j];
-                }
-            }
-        };
-        Float16 s[CB];
 #pragma unroll
         for (int cb = 0; cb < CB; ++cb) {
             float b[16];
             if constexpr (folded) {
                 int row0 = r0;
                 pin(row0);   // loads of its own for each: copies would take an instruction per score
-                shifts(b, row0);
+                shifts(b, buf, row0);
             }
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -629,13 +628,17 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                 s[cb] = product<P>(x, own[cb][ks], s[cb]);
             }
         }
+    };
+    auto use = [&](auto shiftedC, Float16 (&s)[CB], int buf, int r0, int rowBase) {
+        constexpr bool shifted = decltype(shiftedC)::value;
+        constexpr bool folded = shifted && kFold;
         // register i of a lane holds matrix row 8 (i / 4) + 4 half + i % 4, owner row ownBase + cb * 32 + col
         if constexpr (PASS == kLossForward) {
             float b[16];
             float most = 0.0f;   // largest shift
             constexpr bool add = shifted && !folded;
             if constexpr (add) {
-                shifts(b, r0);
+                shifts(b, buf, r0);
                 most = b[0];
 #pragma unroll
                 for (int i = 1; i < 16; ++i) {
@@ -674,7 +677,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                 float b[16];
                 constexpr bool add = shifted && !folded;
                 if constexpr (add) {
-                    shifts(b, r0);
+                    shifts(b, buf, r0);
                 }
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
@@ -699,7 +702,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                 // |grad scale| is in the exponent; its sign, and the 1 at the target, are rarely asked for
                 float shift[16];
                 if constexpr (!folded) {
-                    shifts(shift, r0);
+                    shifts(shift, buf, r0);
                 }
                 hit = __any((unsigned)(auxT[buf][r0 + col] - ownBase) < (unsigned)RW);
                 // four rows' targets and |grad scale|, all loaded: a load of what a comparison asks for would wait for it
@@ -840,6 +843,10 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
         }
     };
 
+    // Both pieces' scores first: the second's products run beside the first's exponentials (2048 x 1 M x 128 bfloat16: dx 990 and
+    // 953 us, dt 1126 and 1067).  Where a piece's scores take 32 registers, or float32's planes many (2048 x 100 k x 64, dx: 175
+    // and 191 us), there is no room for two.
+    constexpr bool kPaired = P == 1 && PASS != kLossForward && TR == 64 && OW == 4 && RW == 32 && DP <= 128;
     auto sweep = [&](auto shiftedC, int from, int to) {
 #pragma unroll 1
         for (int t = from; t < to; ++t) {
@@ -850,10 +857,21 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
                 fetch(t + 1);
             }
             // no condition around the pieces: a wave without rows of its own, or rows past the stream's end, compute zeros
+            if constexpr (kPaired) {
+                Float16 s0[CB];
+                Float16 s1[CB];
+                score(shiftedC, s0, buf, 0);
+                score(shiftedC, s1, buf, 32);
+                use(shiftedC, s0, buf, 0, t * TR);
+                use(shiftedC, s1, buf, 32, t * TR + 32);
+            } else {
 #pragma unroll 1
-            for (int k = 0; k < TR / 32 / L::kStreamWaves; ++k) {
-                const int r0 = (k * L::kStreamWaves + streamWave) * 32;
-                piece(shiftedC, buf, r0, t * TR + r0);
+                for (int k = 0; k < TR / 32 / L::kStreamWaves; ++k) {
+                    const int r0 = (k * L::kStreamWaves + streamWave) * 32;
+                    Float16 s[CB];
+                    score(shiftedC, s, buf, r0);
+                    use(shiftedC, s, buf, r0, t * TR + r0);
+                }
             }
             if (NB == 1) {
                 __syncthreads();
