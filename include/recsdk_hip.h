@@ -769,7 +769,8 @@ RECSDK_API int recsdk_layer_norm_backward(const void* d_grad, const void* d_x, i
  *   d_loss, d_lse  [rows] fp32; d_lse is for the backward pass: log-sum-exp, or +infinity where a row gives no gradient
  *   scale          finite; for bf16 rows with d_item_bias 0, or at least 2^-40 in size
  * d_x, d_table, d_workspace, and the gradients d_dx and d_dtable are 16-byte aligned.  rows and items < 2^30, items >= 1.
- * Rows that are no whole 16-byte pieces, or more than 2^22 elements apart, are copied into the workspace first.
+ * Rows more than 2^22 elements apart, and rows that are no whole 16-byte pieces, are copied into the workspace first, the
+ * table's of 8 and more columns only where x has more than 4096 rows; others are read as they lie.
  * Sums and statistics are fp32.  The gradients take (probability - [target]) grad in the operands' precision: bf16 in one
  * rounding, and a second one of what the first has left where a target is among 32 rows at a time.  fp32 products of more
  * than 32 rows keep 22 bits of each value, and of an operand nothing below 2^-40 of its largest finite one, in rows and items that

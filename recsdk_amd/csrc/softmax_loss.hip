@@ -8,6 +8,8 @@ namespace recsdk {
 
 constexpr int kFewRows = 32;
 constexpr int kAbsMaxThreads = 1024;
+constexpr int kDirectDim = 8;
+constexpr int kDirectRows = 4096;
 constexpr int64_t kMostBlocks = 65536;   // of the kernels here, which walk what is more: a launch holds fewer than 2^32 threads
 
 // Joins the parts of the running sums and takes the target's score off.  TEAM threads per row of x: a wave, or the block
@@ -168,19 +170,21 @@ __global__ __launch_bounds__(kAbsMaxThreads) void k_abs_max(const float* __restr
     __shared__ float sums[kAbsMaxThreads / kWave];
     constexpr int kStep = kAbsMaxParts * (kAbsMaxThreads / 32);
     constexpr int kFlight = 4;   // rows whose loads are in flight at once
+    typedef float Unaligned __attribute__((ext_vector_type(4), aligned(4)));
     const bool second = blockIdx.x >= kAbsMaxParts;
     const float* base = second ? table : x;
     const int64_t stride = second ? tableStride : xStride;
     const int count = second ? items : rows;
     float most = 0.0f;
     for (int r0 = blockIdx.x % kAbsMaxParts * (kAbsMaxThreads / 32) + threadIdx.x / 32; r0 < count; r0 += kFlight * kStep) {
-        for (int c = threadIdx.x % 32 * 4; c < dim; c += 128) {
+        for (int at = threadIdx.x % 32 * 4; at < dim; at += 128) {
+            const int c = dim < 4 ? at : min(at, dim - 4);   // a row's last four columns, where it ends inside a piece
             Float4 v[kFlight];
             bool live[kFlight];
 #pragma unroll
             for (int q = 0; q < kFlight; ++q) {
                 const int64_t r = min((int64_t)r0 + (int64_t)q * kStep, (int64_t)count - 1);
-                v[q] = *reinterpret_cast<const Float4*>(base + r * stride + c);
+                v[q] = *reinterpret_cast<const Unaligned*>(base + r * stride + c);
                 live[q] = second ? bias == nullptr || bias[r] > kMaskedBelow : (uint64_t)target[r] < (uint64_t)items;
             }
 #pragma unroll
@@ -267,8 +271,9 @@ struct LossPlan {
     int planes;
     int bytes;           // of an element
     int padded;          // columns of padded copies
-    bool padX;           // rows that are no whole 16-byte pieces, or too far apart, are copied into padded ones first
+    bool padX;           // rows that are copied into padded ones first
     bool padTable;
+    bool tail;           // the table's rows, not copied, end inside a 16-byte piece
     PassPlan forward, dx, dt;
     int64_t atX, atTable, atMax, atParts;   // offsets into the workspace
     int64_t forwardBytes, backwardBytes;
@@ -276,6 +281,11 @@ struct LossPlan {
 
 static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 
+// The table's rows of eight columns and more are read as they lie, on whatever border they start, for up to kDirectRows rows of x:
+// then the copy takes longer than moving the columns to their places in every tile (1 x 228899 x 203 float32, forward: 149 us with
+// a padded copy, 79 without; 1000 x 100000 x 201 bfloat16: 82 and 67; 4000 x 50000 x 201: 108 and 109, with dx 304 and 312, dt
+// 259 and 247).  x, whose rows every split and every block of items reads again, is always copied (301 x 30011 x 201 bfloat16,
+// forward: 28 us read off the borders, 24 with the copy).
 static LossPlan plan_loss(int64_t rows, int64_t items, int32_t dim, int32_t dtype, int64_t x_stride, int64_t table_stride)
 {
     LossPlan p{};
@@ -285,6 +295,10 @@ static LossPlan plan_loss(int64_t rows, int64_t items, int32_t dim, int32_t dtyp
     p.padded = (int)(cdiv(dim, piece) * piece);
     p.padX = dim % piece != 0 || x_stride % piece != 0 || x_stride > kLossMaxStride;
     p.padTable = dim % piece != 0 || table_stride % piece != 0 || table_stride > kLossMaxStride;
+    if (rows <= kDirectRows && (dim >= kDirectDim || dim % piece == 0) && table_stride <= kLossMaxStride) {
+        p.padTable = false;
+    }
+    p.tail = !p.padTable && dim % piece != 0;
     p.forward = plan_pass(p.planes, dim, rows, items, kLossForward);
     p.dx = plan_pass(p.planes, dim, rows, items, kLossDx);
     p.dt = plan_pass(p.planes, dim, items, rows, kLossDt);
@@ -430,6 +444,7 @@ static int run_forward(const LossPlan& plan, LossOperands o, int64_t rows, int64
     a.owners = (int32_t)rows;
     a.streams = (int32_t)items;
     a.dim = dim;
+    a.tail = plan.tail;
     a.target = target;
     a.bias = bias;
     a.scale = scale;
@@ -473,6 +488,7 @@ static int run_backward(const LossPlan& plan, LossOperands o, int64_t rows, int6
     const float* tableMax = xMax + kAbsMaxParts;
     LossArgs a{};
     a.dim = dim;
+    a.tail = plan.tail;
     a.target = target;
     a.bias = bias;
     a.lse = lse;

@@ -77,6 +77,7 @@ struct LossArgs {
     float* part;            // backward: [split parts][owners past the whole blocks][partDim] partial sums
     int32_t partDim;        // dim rounded up to whole fours
     void* out;              // dt: [owners][dim] in the operands' type, by the whole blocks
+    int32_t tail;           // the table's rows end inside a 16-byte piece (and are no padded copies)
     const float* ownMax;    // P = 2: [kAbsMaxParts] largest values of the operands' rows
     const float* streamMax;
 };
@@ -234,19 +235,43 @@ __device__ __forceinline__ Float16 product(const Frag<P> (&a)[P], const Frag<P> 
     return multiply(a[0], b[0], c);
 }
 
-// Eight columns of a row as they come from memory.  `at` is the first of them, `cols` how many the row has from there on
-// (none, or whole 16-byte pieces); what is not loaded keeps its value.
+// By value: `c ? a[i] : a[j]` of array elements would choose between addresses, and keep the array in memory.
+template <typename V>
+__device__ __forceinline__ V choose(bool c, V a, V b)
+{
+    return c ? a : b;
+}
+
+// Eight columns of a row as they come from memory.  `at` is the first of them, `cols` how many the row has from there on;
+// what is not loaded keeps its value.  Pieces of 16 bytes are loaded whole: where the row ends inside one, `at` lies `back`(cols)
+// columns further back, so that the piece ends where the row does, and `settle` moves the columns to their places.  (Rows have
+// eight columns at least, so what lies further back is the row's own.)  Rows may start on any element.
 template <int P>
 struct RowChunk {
     static constexpr int kBytes = 32;
+    static constexpr int kPiece = 4;   // columns
+    typedef float Piece __attribute__((ext_vector_type(4), aligned(4)));
     Float4 v[2];
     __device__ __forceinline__ void load(const char* at, int cols)
     {
         if (cols > 0) {
-            v[0] = *reinterpret_cast<const Float4*>(at);
+            v[0] = *reinterpret_cast<const Piece*>(at);
         }
         if (cols > 4) {
-            v[1] = *reinterpret_cast<const Float4*>(at + 16);
+            v[1] = *reinterpret_cast<const Piece*>(at + 16);
+        }
+    }
+    __device__ __forceinline__ void settle(int back)
+    {
+        const bool two = (back & 2) != 0;
+        const bool one = (back & 1) != 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j / 4][j % 4] = choose(two, j + 2 < 8 ? v[(j + 2) / 4 % 2][(j + 2) % 4] : 0.0f, v[j / 4][j % 4]);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j / 4][j % 4] = choose(one, j + 1 < 8 ? v[(j + 1) / 4 % 2][(j + 1) % 4] : 0.0f, v[j / 4][j % 4]);
         }
     }
     __device__ __forceinline__ void clear() { v[0] = v[1] = Float4{0, 0, 0, 0}; }
@@ -266,17 +291,35 @@ struct RowChunk {
 template <>
 struct RowChunk<1> {
     static constexpr int kBytes = 16;
+    static constexpr int kPiece = 8;
+    typedef uint32_t Piece __attribute__((ext_vector_type(4), aligned(2)));
     Word4 v;
     __device__ __forceinline__ void load(const char* at, int cols)
     {
         if (cols > 0) {
-            v = *reinterpret_cast<const Word4*>(at);
+            v = *reinterpret_cast<const Piece*>(at);
         }
+    }
+    __device__ __forceinline__ void settle(int back)
+    {
+        const bool four = (back & 4) != 0;
+        const bool two = (back & 2) != 0;
+        const bool one = (back & 1) != 0;
+        v = Word4{choose(four, v[2], v[0]), choose(four, v[3], v[1]), choose(four, 0u, v[2]), choose(four, 0u, v[3])};
+        v = Word4{choose(two, v[1], v[0]), choose(two, v[2], v[1]), choose(two, v[3], v[2]), choose(two, 0u, v[3])};
+        v = Word4{choose(one, v[0] >> 16 | v[1] << 16, v[0]), choose(one, v[1] >> 16 | v[2] << 16, v[1]),
+                  choose(one, v[2] >> 16 | v[3] << 16, v[2]), choose(one, v[3] >> 16, v[3])};
     }
     __device__ __forceinline__ void clear() { v = Word4{0, 0, 0, 0}; }
     __device__ __forceinline__ void negate() { v ^= Word4{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u}; }
     __device__ __forceinline__ void planes(Frag<1> (&p)[1], float) const { __builtin_memcpy(&p[0], &v, 16); }
 };
+
+template <int P>
+__device__ __forceinline__ int back(int cols)
+{
+    return cols > 0 && cols < 8 ? -cols & (RowChunk<P>::kPiece - 1) : 0;
+}
 
 __device__ __forceinline__ float wave_max(float v)
 {
@@ -385,9 +428,13 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
-            const int c = (ks * 2 + half) * 8;
+            int c = (ks * 2 + half) * 8;
+            const int cols = a.dim - c;
+            if (kDt && a.tail != 0) {
+                c -= back<P>(cols);
+            }
             ownRaw[cb][ks].clear();
-            ownRaw[cb][ks].load(static_cast<const char*>(a.own) + (n * a.ownStride * kElement + c * kElement), a.dim - c);
+            ownRaw[cb][ks].load(static_cast<const char*>(a.own) + (n * a.ownStride * kElement + c * kElement), cols);
         }
     }
 
@@ -398,7 +445,9 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
     const int chunkRow = threadIdx.x / CH;
     const int chunkCols = a.dim - chunk * 8;
     const int64_t strideBytes = a.streamStride * kElement;
-    const uint32_t chunkAt = (uint32_t)(chunkRow * strideBytes + chunk * RowChunk<P>::kBytes);
+    const int chunkBack = !kDt && a.tail != 0 ? back<P>(chunkCols) : 0;
+    const int chunkByte = chunk * RowChunk<P>::kBytes - chunkBack * kElement;
+    const uint32_t chunkAt = (uint32_t)(chunkRow * strideBytes + chunkByte);
     float ownScale = 1.0f;
     float streamScale = 1.0f;
     RowChunk<P> staged[L::kLoads];
@@ -418,7 +467,7 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
 #pragma unroll
             for (int q = 0; q < L::kLoads; ++q) {
                 const int r = min(q * kStep + chunkRow, last);
-                staged[q].load(base + (int64_t)r * strideBytes + chunk * RowChunk<P>::kBytes, chunkCols);
+                staged[q].load(base + (int64_t)r * strideBytes + chunkByte, chunkCols);
             }
         }
     };
@@ -472,6 +521,12 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
         }
     };
     auto place = [&](int buf, int t, const Aux& x) {
+        if (!kDt && a.tail != 0) {
+#pragma unroll
+            for (int q = 0; q < L::kLoads; ++q) {
+                staged[q].settle(chunkBack);
+            }
+        }
         if constexpr (kMasks) {
             uint32_t any = 0;
 #pragma unroll
@@ -558,6 +613,9 @@ __global__ __launch_bounds__(kLossThreads, loss_waves(P, DP, OW, PASS)) void k_s
         }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
+            if (kDt && a.tail != 0) {
+                ownRaw[cb][ks].settle(back<P>(a.dim - (ks * 2 + half) * 8));
+            }
             if (!live || still) {
                 ownRaw[cb][ks].clear();   // rows past the end, padding positions and free slots may hold anything
             }

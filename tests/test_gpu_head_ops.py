@@ -672,6 +672,31 @@ def test_softmax_loss_large_table_and_no_rows(ops):
 
 
 @pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [8, 9, 10, 11, 12, 13, 14, 15, 31, 67, 125, 254])
+def test_softmax_loss_rows_that_end_inside_a_piece(ops, kind, dim):
+    # tables whose last row ends with the allocation, at each place in a 16-byte piece; strides of no whole pieces
+    x, table, target, grad = loss_case(45, 130, dim, kind, 300 + dim)
+    check_loss(ops, x, table, target, None, 3 / math.sqrt(dim), grad)
+    wide = torch.full((130, dim + 3), math.nan, dtype=TYPES[kind], device=DEV)
+    wide[:, :dim] = table
+    check_loss(ops, x, wide[:, :dim], target, None, 3 / math.sqrt(dim), grad)   # what lies behind a row is not looked at
+    few = torch.full((45, dim + 5), math.inf, dtype=TYPES[kind], device=DEV)
+    few[:, :dim] = x
+    check_loss(ops, few[:, :dim], table, target, None, 3 / math.sqrt(dim), grad)
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,items", [(1030, 140_000), (5000, 3000)])   # a table read as it lies, and one that is copied
+def test_softmax_loss_rows_off_the_borders_are_read_as_padded_ones(ops, kind, rows, items):
+    x, table, target, grad = loss_case(rows, items, 250, kind, 97)
+    leaves = [t.detach().requires_grad_() for t in (x, table)]
+    dx, dt = torch.autograd.grad(ops.softmax_loss(*leaves, target, None, 0.2), leaves, grad)
+    padded = [torch.nn.functional.pad(t.detach(), (0, 6)).requires_grad_() for t in (x, table)]
+    px, pt = torch.autograd.grad(ops.softmax_loss(*padded, target, None, 0.2), padded, grad)
+    assert torch.equal(dx, px[:, :250]) and torch.equal(dt, pt[:, :250])
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
 def test_softmax_loss_rows_far_apart(ops, kind):
     x, table, target, grad = loss_case(5, 9, 64, kind, 96)
     far = torch.zeros(9, 2 ** 22 + 8, dtype=TYPES[kind], device=DEV)

@@ -103,8 +103,12 @@ def test_softmax_loss_workspace_grows_with_what_is_copied():
     L, f, b = capi.lib(), ctypes.c_int64(), ctypes.c_int64()
     assert L.recsdk_softmax_loss_workspace(100, 1000, 64, BF16, 64, 64, f, b) == capi.OK
     plain = f.value, b.value
-    assert L.recsdk_softmax_loss_workspace(100, 1000, 64, BF16, 64, 65, f, b) == capi.OK   # table rows off the 16-byte border
-    assert f.value >= plain[0] + 1000 * 64 * 2 and b.value >= plain[1] + 1000 * 64 * 2
+    assert L.recsdk_softmax_loss_workspace(100, 1000, 64, BF16, 64, 65, f, b) == capi.OK   # off the 16-byte border: read as they are
+    assert (f.value, b.value) == plain
+    assert L.recsdk_softmax_loss_workspace(100, 1000, 8, BF16, 8, 8, f, b) == capi.OK
+    plain = f.value, b.value
+    assert L.recsdk_softmax_loss_workspace(100, 1000, 7, BF16, 7, 7, f, b) == capi.OK   # shorter than a 16-byte piece: copied
+    assert f.value >= plain[0] + 1000 * 8 * 2 and b.value >= plain[1] + 1000 * 8 * 2
     assert L.recsdk_softmax_loss_workspace(0, 1000, 64, BF16, 64, 64, f, b) == capi.OK and f.value == b.value == 0
 
 
