@@ -226,18 +226,19 @@ static PassPlan plan_pass(int planes, int dim, int64_t owners, int64_t streams, 
     PassPlan p{};
     p.rowsPerWave = wide_rows(planes, dp, pass);
     p.ownWaves = 4;
-    if (pass != kLossDt) {
-        if (owners <= 128) {
-            p.rowsPerWave = 32;
-        }
-        if (owners <= kFewRows) {
-            p.ownWaves = narrow_waves(planes, dp);
-        }
+    // Smaller blocks where there are few: a wave's 32 rows instead of 64 (bfloat16 x 64, dx, 300 x 30000: 21 us with 64 rows, 18
+    // with 32; 8192 x 200003: 504 and 532; dt, 300 x 30000: 17 and 11, 2000 x 100000: 84 and 72, 8000 x 60000: 171 and 175;
+    // x 96, 4000 x 130000: 219 and 235).
+    if (owners <= (pass == kLossForward ? 128 : pass == kLossDx ? 1024 : streams <= 2048 ? 131072 : 32768)) {
+        p.rowsPerWave = 32;
+    }
+    if (pass != kLossDt && owners <= kFewRows) {
+        p.ownWaves = narrow_waves(planes, dp);
     }
     p.blocks = cdiv(owners, (int64_t)p.rowsPerWave * p.ownWaves);
     const int tileRows = tile_rows(planes, dp, p.ownWaves, pass);
     const int64_t tiles = cdiv(streams, tileRows);
-    const int64_t resident = (int64_t)kComputeUnits * resident_blocks(planes, dp, pass);
+    const int64_t resident = (int64_t)kComputeUnits * resident_blocks(planes, dp, pass, p.rowsPerWave);
     const int64_t most = tiles < kSplitTiles ? 1 : tiles / kSplitTiles;
     int64_t splits = std::clamp(resident / p.blocks, (int64_t)1, most);
     if (pass == kLossDt && splits == 1) {

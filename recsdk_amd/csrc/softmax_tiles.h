@@ -129,8 +129,11 @@ constexpr int loss_waves(int planes, int dp, int ownWaves, int pass)
 }
 
 // Blocks that a compute unit holds at once, by the registers and LDS of the kernels.
-constexpr int resident_blocks(int planes, int dp, int pass)
+constexpr int resident_blocks(int planes, int dp, int pass, int rowsPerWave)
 {
+    if (pass != kLossForward && rowsPerWave < wide_rows(planes, dp, pass)) {
+        return dp <= 64 ? 3 : 2;
+    }
     if (pass == kLossForward) {
         return planes == 1   ? (dp <= 64 ? 4 : dp <= 128 ? 3 : dp <= 224 ? 2 : 1)
                : planes == 2 ? (dp <= 64 ? 4 : dp <= 128 ? 3 : 2)
@@ -1021,8 +1024,12 @@ int launch_width(const LossArgs& a, const PassPlan& p, hipStream_t stream)
             return launch_tiles<P, DP, 32, narrow_waves(P, DP), PASS, true>(a, p, stream);
         }
     }
-    if constexpr (PASS != kLossDt && kWide == 64) {
+    if constexpr (kWide == 64) {
         if (p.rowsPerWave == 32) {
+            if constexpr (PASS == kLossDt) {   // a shift is an item's own there, and costs nothing to do without
+                return a.bias != nullptr ? launch_tiles<P, DP, 32, 4, PASS, true>(a, p, stream)
+                                         : launch_tiles<P, DP, 32, 4, PASS, false>(a, p, stream);
+            }
             return launch_tiles<P, DP, 32, 4, PASS, true>(a, p, stream);
         }
     }
